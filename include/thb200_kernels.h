@@ -322,6 +322,32 @@ int thb_to_nchw(int dtype, const void *x, int N, int H, int W, int C, int x_ld, 
 #define THB_STATIC_CSUM_MAX_PIXELS 1048576
 int thb_conv_u8_fwd_static(const thb_conv_desc *d, const void *x, void *y, thb_stream s);
 
+/* ------------------------------------------------------------------------------------------
+ * A decoder's step on new tokens.  No counterpart in the reference.  Rows are tokens: row r of a tensor starts r * ld
+ * elements behind its base; ld is a multiple of thb_channel_align(dtype) (16 for 8-bit values), bases are 16-byte aligned.
+ * Sums, norms and softmax statistics are fp32.  Everything that can be seen from the arguments is checked before
+ * the launch (THB_ERR_ARG: out of range or missing; THB_ERR_UNSUPPORTED: no kernel for it; the reason is in
+ * thb_last_cuda_error()); an empty call (no rows, no tokens) launches nothing and succeeds.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Root-mean-square norm of x + res:
+ *     t = x + res (res NULL: t = x);  sum = t;  v = t / sqrt(mean(t^2) + eps) * gain;  y = v;  q = e4m3(v / q_scale),
+ *     q_scale = max|v| / 448 of the row.
+ * sum, y and q (with q_scale) are optional, one of them at least is given; the norm is taken from t before it is rounded for
+ * `sum`.  sum, y may be x or res themselves.  Values behind C up to the next multiple of the alignment are ignored in x and
+ * res and written as zeros.  A row whose v are all below 2^-100 has q_scale = 0 and zeros in q; one with an infinite or NaN t, or a
+ * norm beyond fp32's range, has q_scale = NaN.  C <= 32768. */
+typedef struct thb_rmsnorm_desc {
+    int dtype; /* F32 / F16 / BF16: of x, res, sum, y */
+    int C;
+    long rows;
+    int x_ld, res_ld, sum_ld, y_ld, q_ld;
+    const float *gain; /* [C]; NULL: ones */
+    float eps;         /* >= 0 */
+} thb_rmsnorm_desc;
+int thb_rmsnorm_fwd(const thb_rmsnorm_desc *d, const void *x, const void *res, void *sum, void *y, void *q, float *q_scale,
+                    thb_stream s);
+
 /* the launchers read their diagnostic THB200_* environment switches once; this re-reads them */
 void thb_conv_reload_knobs(void);
 const char *thb_last_cuda_error(void);

@@ -54,6 +54,12 @@ class ConvDesc(C.Structure):
     ]
 
 
+class RmsNormDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("C", C.c_int), ("rows", C.c_long),
+                ("x_ld", C.c_int), ("res_ld", C.c_int), ("sum_ld", C.c_int), ("y_ld", C.c_int), ("q_ld", C.c_int),
+                ("gain", C.c_void_p), ("eps", C.c_float)]
+
+
 def aligned_tmap():
     """A 64-byte aligned thb_tmap plus the buffer that keeps it alive."""
     raw = (C.c_ubyte * (128 + 64))()
@@ -98,6 +104,7 @@ def load(libpath: str | None = None):
     lib.thb_col2im.argtypes = [ci, vp] + [ci] * 13 + [cf, vp, C.POINTER(Act), vp, ci, vp]
     lib.thb_u8_channel_sum.argtypes = [vp, cl, ci, ci, vp, vp]
     lib.thb_to_nchw.argtypes = [ci, vp, ci, ci, ci, ci, ci, vp, vp]
+    lib.thb_rmsnorm_fwd.argtypes = [C.POINTER(RmsNormDesc), vp, vp, vp, vp, vp, vp, vp]
     lib.thb_last_cuda_error.restype = C.c_char_p
     lib.thb_kernel_launch_count.restype = ci
     return lib
