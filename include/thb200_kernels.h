@@ -348,6 +348,34 @@ typedef struct thb_rmsnorm_desc {
 int thb_rmsnorm_fwd(const thb_rmsnorm_desc *d, const void *x, const void *res, void *sum, void *y, void *q, float *q_scale,
                     thb_stream s);
 
+/* Linear with 4-bit weights on N <= 8 rows, weights read once (thb_gemv_fwd with codes and scales in place of the weights):
+ *     y[n][m] = act(scale[m] * x_scale[n] * sum_k x[n][k] * (code[m][k] - zero[m][k / group]) * wscale[m][k / group] + shift[m])
+ * code[m][k] is the low (k even) or high (k odd) nibble of byte k / 2 of row m of w.  x has the descriptor's dtype, or, where
+ * x_scale is given, e4m3 codes with a scale a row, as thb_rmsnorm_fwd leaves them (and a dtype of y of any of the three).
+ * Products are exact (fp32 x: in three parts), sums fp32.  What lies behind K in x and w is ignored; values of y behind M up
+ * to the next multiple of the alignment are written as zeros.  w, wscale and wzero are read ahead of the launches before this
+ * one in the stream that are still running: nothing in this library writes them. */
+typedef struct thb_gemv_q4_desc {
+    int dtype; /* F32 / F16 / BF16: of y, and of x without x_scale */
+    int N, K, M;
+    int group;                  /* weights a scale: 32, 64 or 128 */
+    int x_ld, y_ld;
+    int w_ld;                   /* bytes a row of w, a multiple of 16 */
+    int s_ld, z_ld;             /* entries a row of wscale and wzero */
+    int wscale_dtype;           /* F32 / F16 / BF16 */
+    const unsigned char *w;     /* [M][w_ld] */
+    const void *wscale;         /* [M][s_ld] */
+    const unsigned char *wzero; /* [M][z_ld], 0..15 (the low four bits are taken); NULL: 8 everywhere */
+    const float *scale, *shift; /* [M]; NULL: 1 / 0 */
+    thb_act act;
+} thb_gemv_q4_desc;
+int thb_gemv_q4_fwd(const thb_gemv_q4_desc *d, const void *x, const float *x_scale, void *y, thb_stream s);
+/* Host-side: rows of fp32 weights (ld floats apart) to nearest codes, scales and, with_zero != 0, zero points (else codes 1..15
+ * around 8; wzero may be NULL).  Scales are what a caller rounds further if wscale_dtype is to be a 16-bit type.  Every pointer is a
+ * HOST pointer; weights that are not finite are refused. */
+int thb_q4_quantize_host(const float *w_host, long M, int K, long ld, int group, int with_zero, unsigned char *codes_host, int w_ld,
+                         float *wscale_host, int s_ld, unsigned char *wzero_host, int z_ld);
+
 /* the launchers read their diagnostic THB200_* environment switches once; this re-reads them */
 void thb_conv_reload_knobs(void);
 const char *thb_last_cuda_error(void);

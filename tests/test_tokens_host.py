@@ -44,3 +44,53 @@ def test_rmsnorm_refusals(lib):
                 dict(q_scale=None), dict(total=None, y=None, q=None, q_scale=None)):
         assert call(norm_desc(), **bad) == ARG, bad
     assert call(changed(norm_desc, rows=0)) == OK
+
+
+def q4_desc():
+    return K.GemvQ4Desc(dtype=K.THB_F16, N=2, K=100, M=30, group=32, x_ld=104, y_ld=32, w_ld=64, s_ld=4, z_ld=4, wscale_dtype=K.THB_F16,
+                        w=AT, wscale=AT, wzero=AT)
+
+
+def test_gemv_q4_refusals(lib):
+    def call(d, x=AT, x_scale=None, y=AT):
+        return lib.thb_gemv_q4_fwd(C.byref(d), x, x_scale, y, None)
+
+    assert lib.thb_gemv_q4_fwd(None, AT, None, AT, None) == ARG
+    for bad in (dict(dtype=K.THB_U8), dict(dtype=9), dict(N=9), dict(group=16), dict(group=0), dict(group=256), dict(wscale_dtype=K.THB_U8)):
+        assert call(changed(q4_desc, **bad)) == UNSUPPORTED, bad
+    for bad in (dict(N=-1), dict(K=0), dict(M=0), dict(x_ld=96), dict(x_ld=101), dict(y_ld=24), dict(y_ld=31), dict(w_ld=48), dict(w_ld=56),
+                dict(s_ld=3), dict(z_ld=3), dict(w=None), dict(w=AT + 8), dict(wscale=None), dict(wscale=AT + 1),
+                dict(act=K.Act(kind=6)), dict(act=K.Act(kind=-1)), dict(act=K.Act(kind=K.ACT_PRELU))):
+        assert call(changed(q4_desc, **bad)) == ARG, bad
+    for bad in (dict(x=None), dict(y=None), dict(x=AT + 8), dict(y=AT + 4), dict(x_scale=AT)):  # (with scales x_ld is a multiple of 16)
+        assert call(q4_desc(), **bad) == ARG, bad
+    assert call(changed(q4_desc, N=0)) == OK
+
+
+@pytest.mark.parametrize("with_zero", [0, 1])
+@pytest.mark.parametrize("k,group", [(1, 32), (100, 32), (257, 128), (64, 64)])
+def test_q4_quantize_host(lib, with_zero, k, group):
+    """The nearest code of every weight: half a step off at most, and the ends of a group are reached."""
+    import numpy as np
+    rng = np.random.default_rng(k)
+    w = (rng.standard_normal((7, k + 3)) * np.exp(rng.standard_normal((7, 1)))).astype(np.float32)
+    w[3, :k] = 0
+    w[4, :k] = np.abs(w[4, :k])
+    groups, ld = (k + group - 1) // group, (k + 1) // 2 + 5
+    codes, s, z = np.full((7, ld), 255, np.uint8), np.full((7, groups + 1), 9, np.float32), np.full((7, groups + 2), 77, np.uint8)
+    at = lambda a: a.ctypes.data  # noqa: E731
+    assert lib.thb_q4_quantize_host(at(w), 7, k, k + 3, group, with_zero, at(codes), ld, at(s), groups + 1, at(z), groups + 2) == OK
+    q = np.stack((codes & 15, codes >> 4), 2).reshape(7, -1)[:, :k].astype(np.float64)
+    wide = lambda a: np.repeat(a[:, :groups], group, 1)[:, :k].astype(np.float64)  # noqa: E731
+    zero = wide(z) if with_zero else 8.0
+    got = (q - zero) * wide(s)
+    # half a step, and where the zero point itself was rounded a range's end may be half a step beyond the last code
+    assert np.all(np.abs(got - w[:, :k]) <= wide(s) * (1.0 if with_zero else 0.5) * (1 + 1e-6))
+    assert np.all(s[:, groups] == 9) and np.all(z[:, groups:] == 77) and (with_zero or np.all(z == 77))
+    assert np.all(got[3] == 0) and (with_zero or q.min() >= 1)
+    w[0, 0] = np.inf
+    assert lib.thb_q4_quantize_host(at(w), 7, k, k + 3, group, with_zero, at(codes), ld, at(s), groups + 1, at(z), groups + 2) == ARG
+    for bad in ((None, 7, k, k + 3, group, 1, at(codes), ld, at(s), groups, at(z), groups), (at(w), 7, k, k - 1, group, 1, at(codes), ld, at(s), groups, at(z), groups),
+                (at(w), 7, k, k, group, 1, at(codes), (k + 1) // 2 - 1, at(s), groups, at(z), groups), (at(w), 7, k, k, group, 1, at(codes), ld, at(s), groups, None, groups),
+                (at(w), 7, k, k, group, 1, at(codes), ld, at(s), groups - 1, at(z), groups), (at(w), 7, k, k, 0, 1, at(codes), ld, at(s), groups, at(z), groups)):
+        assert lib.thb_q4_quantize_host(*bad) == ARG

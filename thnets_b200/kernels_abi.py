@@ -60,6 +60,13 @@ class RmsNormDesc(C.Structure):
                 ("gain", C.c_void_p), ("eps", C.c_float)]
 
 
+class GemvQ4Desc(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("N", C.c_int), ("K", C.c_int), ("M", C.c_int), ("group", C.c_int),
+                ("x_ld", C.c_int), ("y_ld", C.c_int), ("w_ld", C.c_int), ("s_ld", C.c_int), ("z_ld", C.c_int),
+                ("wscale_dtype", C.c_int), ("w", C.c_void_p), ("wscale", C.c_void_p), ("wzero", C.c_void_p),
+                ("scale", C.c_void_p), ("shift", C.c_void_p), ("act", Act)]
+
+
 def aligned_tmap():
     """A 64-byte aligned thb_tmap plus the buffer that keeps it alive."""
     raw = (C.c_ubyte * (128 + 64))()
@@ -105,6 +112,8 @@ def load(libpath: str | None = None):
     lib.thb_u8_channel_sum.argtypes = [vp, cl, ci, ci, vp, vp]
     lib.thb_to_nchw.argtypes = [ci, vp, ci, ci, ci, ci, ci, vp, vp]
     lib.thb_rmsnorm_fwd.argtypes = [C.POINTER(RmsNormDesc), vp, vp, vp, vp, vp, vp, vp]
+    lib.thb_gemv_q4_fwd.argtypes = [C.POINTER(GemvQ4Desc), vp, vp, vp, vp]
+    lib.thb_q4_quantize_host.argtypes = [vp, cl, ci, cl, ci, ci, vp, ci, vp, ci, vp, ci]
     lib.thb_last_cuda_error.restype = C.c_char_p
     lib.thb_kernel_launch_count.restype = ci
     return lib
