@@ -376,6 +376,53 @@ int thb_gemv_q4_fwd(const thb_gemv_q4_desc *d, const void *x, const float *x_sca
 int thb_q4_quantize_host(const float *w_host, long M, int K, long ld, int group, int with_zero, unsigned char *codes_host, int w_ld,
                          float *wscale_host, int s_ld, unsigned char *wzero_host, int z_ld);
 
+/* Keys and values of many sequences in pages of one pool.  Value c of head h of token i of page p is element
+ * p * page_stride + i * token_stride + h * head_stride + c of k and of v: [pages][page_len][heads][dim] and
+ * [pages][heads][page_len][dim] are both such layouts.  Position j of sequence b is token j % page_len of page
+ * table[b * table_ld + j / page_len].  Pages and sequences are checked on the device: what lies outside the table or the pool is neither
+ * read nor written, and *status becomes THB_ERR_ARG (the caller clears it). */
+typedef struct thb_kv_cache {
+    int dtype;      /* F32 / F16 / BF16 */
+    int heads, dim; /* dim: a multiple of thb_channel_align(dtype), 256 at most */
+    int pages, page_len;
+    long page_stride, token_stride, head_stride; /* elements; multiples of thb_channel_align(dtype) */
+    void *k, *v;
+    const int *table; /* [sequences][table_ld] */
+    int table_ld, sequences;
+    int *status;
+} thb_kv_cache;
+
+/* Rotary positions: pair i of the first `dim` values of a head is turned by pos * freq[i] radians and multiplied by magnitude; the
+ * values behind are copied.  Angles are reduced in fp64. */
+typedef struct thb_rope {
+    int dim;            /* even; 0: no rotation */
+    int interleaved;    /* pairs (2i, 2i + 1); 0: (i, i + dim / 2) */
+    const double *freq; /* device array of dim / 2 */
+    float magnitude;
+} thb_rope;
+/* freq and magnitude of the usual scalings: freq[i] = base^(-2i/dim), and for contexts `factor` times longer than a model was trained for
+ * LINEAR: divided by factor (positions interpolated); BASE: base multiplied by factor^(dim/(dim-2)) (the "NTK-aware" base);
+ * BY_PARTS: divided by factor where a pair makes at most slow_turns turns in trained_len positions, kept where it makes
+ * fast_turns or more, in proportion between, and magnitude 0.1 ln(factor) + 1 (YaRN).  The other scalings' magnitude is 1. */
+enum { THB_ROPE_PLAIN = 0, THB_ROPE_LINEAR = 1, THB_ROPE_BASE = 2, THB_ROPE_BY_PARTS = 3 };
+int thb_rope_freq_host(int dim, double base, int scaling, double factor, double trained_len, double slow_turns, double fast_turns,
+                       double *freq_host, float *magnitude);
+
+/* New tokens into the cache: token t's keys, rotated by pos[t], and its values go to position pos[t] of sequence seq[t]; its queries,
+ * rotated the same, to q_out (which may be q).  k, v, q: rows of heads * dim values (parts of one row of q, k and v side by
+ * side, if the caller likes).  k = v = NULL: only the queries (the cache's dtype and dim are read, no more); q = q_out = NULL: only
+ * the cache.  A token with pos < 0 is a place in a padded batch: nothing of it is read or written.  No two tokens of a call may have the
+ * same position of the same sequence, nor two sequences of a call the same page where both write. */
+typedef struct thb_kv_append_desc {
+    thb_kv_cache cache;
+    thb_rope rope;
+    int tokens;
+    const int *pos; /* [tokens] */
+    const int *seq; /* [tokens]; NULL: token t is of sequence t */
+    int k_ld, v_ld, q_ld, q_out_ld, q_heads;
+} thb_kv_append_desc;
+int thb_kv_append_fwd(const thb_kv_append_desc *d, const void *k, const void *v, const void *q, void *q_out, thb_stream s);
+
 /* the launchers read their diagnostic THB200_* environment switches once; this re-reads them */
 void thb_conv_reload_knobs(void);
 const char *thb_last_cuda_error(void);

@@ -94,3 +94,71 @@ def test_q4_quantize_host(lib, with_zero, k, group):
                 (at(w), 7, k, k, group, 1, at(codes), (k + 1) // 2 - 1, at(s), groups, at(z), groups), (at(w), 7, k, k, group, 1, at(codes), ld, at(s), groups, None, groups),
                 (at(w), 7, k, k, group, 1, at(codes), ld, at(s), groups - 1, at(z), groups), (at(w), 7, k, k, 0, 1, at(codes), ld, at(s), groups, at(z), groups)):
         assert lib.thb_q4_quantize_host(*bad) == ARG
+
+
+def cache_desc(**fields):
+    c = K.KvCache(dtype=K.THB_F16, heads=4, dim=64, pages=10, page_len=16, page_stride=4096, token_stride=256, head_stride=64, k=AT, v=AT,
+                  table=AT, table_ld=5, sequences=3, status=AT)
+    for name, value in fields.items():
+        setattr(c, name, value)
+    return c
+
+
+BAD_CACHES = (dict(heads=0), dict(dim=0), dict(dim=60), dict(dim=264), dict(dim=-64), dict(pages=0), dict(page_len=0), dict(table_ld=0),
+              dict(sequences=0), dict(k=None), dict(v=None), dict(table=None), dict(status=None), dict(k=AT + 8), dict(v=AT + 2),
+              dict(page_stride=4100), dict(token_stride=252), dict(head_stride=60), dict(page_stride=-4096), dict(token_stride=-256),
+              dict(head_stride=-64), dict(token_stride=248), dict(head_stride=56), dict(page_stride=4088), dict(head_stride=128),
+              dict(token_stride=64, head_stride=1016), dict(page_stride=1 << 41), dict(page_len=32))
+
+
+def append_desc():
+    return K.KvAppendDesc(cache=cache_desc(), rope=K.Rope(dim=64, freq=AT, magnitude=1.0), tokens=2, pos=AT, seq=AT, k_ld=256, v_ld=256,
+                          q_ld=512, q_out_ld=512, q_heads=8)
+
+
+def test_kv_append_refusals(lib):
+    def call(d, k=AT, v=AT, q=AT, q_out=AT):
+        return lib.thb_kv_append_fwd(C.byref(d), k, v, q, q_out, None)
+
+    assert lib.thb_kv_append_fwd(None, AT, AT, AT, AT, None) == ARG
+    for dtype in (K.THB_U8, 7):
+        assert call(changed(append_desc, cache=cache_desc(dtype=dtype))) == UNSUPPORTED
+    for bad in BAD_CACHES:
+        assert call(changed(append_desc, cache=cache_desc(**bad))) == ARG, bad
+    for bad in (dict(tokens=-1), dict(pos=None), dict(rope=K.Rope(dim=63, freq=AT)), dict(rope=K.Rope(dim=66, freq=AT)), dict(rope=K.Rope(dim=-2, freq=AT)),
+                dict(rope=K.Rope(dim=64)), dict(q_heads=0), dict(q_ld=504), dict(q_out_ld=516), dict(k_ld=248), dict(v_ld=260), dict(seq=None, tokens=4)):
+        assert call(changed(append_desc, **bad)) == ARG, bad
+    for bad in (dict(k=None), dict(v=None), dict(q=None), dict(q_out=None), dict(k=AT + 8), dict(v=AT + 4), dict(q=AT + 2), dict(q_out=AT + 8),
+                dict(k=None, v=None, q=None, q_out=None)):
+        assert call(append_desc(), **bad) == ARG, bad
+    assert call(changed(append_desc, cache=cache_desc(dim=60)), k=None, v=None) == ARG
+    assert call(changed(append_desc, tokens=0)) == OK
+
+
+def test_rope_freq_host(lib):
+    import math
+
+    import numpy as np
+    out, mag = np.zeros(32), C.c_float()
+
+    def call(dim=64, base=10000.0, scaling=K.ROPE_PLAIN, factor=4.0, trained=4096.0, slow=1.0, fast=32.0):
+        out[:] = -1
+        rc = lib.thb_rope_freq_host(dim, base, scaling, factor, trained, slow, fast, out.ctypes.data, C.byref(mag))
+        return rc, out[: dim // 2].copy() if dim > 0 else None, mag.value
+
+    plain = 10000.0 ** (-np.arange(32) / 32)
+    assert call()[0] == OK and np.allclose(call()[1], plain, rtol=1e-14) and call()[2] == 1.0
+    assert np.allclose(call(scaling=K.ROPE_LINEAR)[1], plain / 4, rtol=1e-14)
+    # the raised base leaves the fastest pair and slows the last one by the whole factor
+    raised = call(scaling=K.ROPE_BASE)[1]
+    assert np.isclose(raised[0], plain[0]) and np.isclose(raised[31], plain[31] / 4) and np.all(np.diff(raised) < 0)
+    rc, parts, m = call(scaling=K.ROPE_BY_PARTS)
+    turns = 4096 * plain / (2 * math.pi)
+    assert rc == OK and np.isclose(m, 0.1 * math.log(4) + 1)
+    assert np.allclose(parts[turns >= 32], plain[turns >= 32]) and np.allclose(parts[turns <= 1], plain[turns <= 1] / 4)
+    assert np.all(parts <= plain * (1 + 1e-12)) and np.all(parts >= plain / 4 * (1 - 1e-12)) and np.all(np.diff(parts) < 0)
+    for bad in (dict(dim=0), dict(dim=63), dict(dim=-2), dict(base=0.0), dict(base=float("nan")), dict(scaling=1, factor=0.5), dict(scaling=2, factor=float("nan")),
+                dict(scaling=3, trained=0.0), dict(scaling=3, slow=32.0), dict(scaling=3, slow=-1.0)):
+        assert call(**bad)[0] == ARG, bad
+    assert call(scaling=4)[0] == UNSUPPORTED and call(scaling=-1)[0] == UNSUPPORTED and call(dim=2, scaling=2)[0] == UNSUPPORTED
+    assert call(dim=2)[0] == OK

@@ -57,3 +57,5 @@ template <typename T, typename T2> struct Vec16Half {
 };
 template <> struct Vec16<__half> : Vec16Half<__half, __half2> {};
 template <> struct Vec16<__nv_bfloat16> : Vec16Half<__nv_bfloat16, __nv_bfloat162> {};
+
+const char *thb_kv_cache_fault(const thb_kv_cache *c);  // kv_append.cu

@@ -11,6 +11,7 @@ import os
 import numpy as np
 
 THB_F32, THB_F16, THB_BF16, THB_U8 = 0, 1, 2, 3
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_BY_PARTS = 0, 1, 2, 3
 ACT_NONE, ACT_THRESHOLD, ACT_LEAKY, ACT_PRELU, ACT_SIGMOID, ACT_TANH = 0, 1, 2, 3, 4, 5
 ESIZE = {THB_F32: 4, THB_F16: 2, THB_BF16: 2, THB_U8: 1}
 ALIGN = {THB_F32: 4, THB_F16: 8, THB_BF16: 8, THB_U8: 16}
@@ -67,6 +68,22 @@ class GemvQ4Desc(C.Structure):
                 ("scale", C.c_void_p), ("shift", C.c_void_p), ("act", Act)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("heads", C.c_int), ("dim", C.c_int), ("pages", C.c_int), ("page_len", C.c_int),
+                ("page_stride", C.c_long), ("token_stride", C.c_long), ("head_stride", C.c_long),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("table_ld", C.c_int), ("sequences", C.c_int),
+                ("status", C.c_void_p)]
+
+
+class Rope(C.Structure):
+    _fields_ = [("dim", C.c_int), ("interleaved", C.c_int), ("freq", C.c_void_p), ("magnitude", C.c_float)]
+
+
+class KvAppendDesc(C.Structure):
+    _fields_ = [("cache", KvCache), ("rope", Rope), ("tokens", C.c_int), ("pos", C.c_void_p), ("seq", C.c_void_p),
+                ("k_ld", C.c_int), ("v_ld", C.c_int), ("q_ld", C.c_int), ("q_out_ld", C.c_int), ("q_heads", C.c_int)]
+
+
 def aligned_tmap():
     """A 64-byte aligned thb_tmap plus the buffer that keeps it alive."""
     raw = (C.c_ubyte * (128 + 64))()
@@ -114,6 +131,8 @@ def load(libpath: str | None = None):
     lib.thb_rmsnorm_fwd.argtypes = [C.POINTER(RmsNormDesc), vp, vp, vp, vp, vp, vp, vp]
     lib.thb_gemv_q4_fwd.argtypes = [C.POINTER(GemvQ4Desc), vp, vp, vp, vp]
     lib.thb_q4_quantize_host.argtypes = [vp, cl, ci, cl, ci, ci, vp, ci, vp, ci, vp, ci]
+    lib.thb_kv_append_fwd.argtypes = [C.POINTER(KvAppendDesc), vp, vp, vp, vp, vp]
+    lib.thb_rope_freq_host.argtypes = [ci, C.c_double, ci, C.c_double, C.c_double, C.c_double, C.c_double, vp, C.POINTER(cf)]
     lib.thb_last_cuda_error.restype = C.c_char_p
     lib.thb_kernel_launch_count.restype = ci
     return lib
