@@ -423,6 +423,28 @@ typedef struct thb_kv_append_desc {
 } thb_kv_append_desc;
 int thb_kv_append_fwd(const thb_kv_append_desc *d, const void *k, const void *v, const void *q, void *q_out, thb_stream s);
 
+/* Attention of one new token a sequence over the cache: row r's queries (q_heads of dim values; query head h reads key head
+ * h / (q_heads / heads)) against positions max(0, len[r] - window) .. len[r] - 1 of sequence seq[r],
+ *     y[h] = sum_j softmax_j(scale * q[h].k[j]) v[j],   lse[r][h] = ln(sum_j exp(scale * q[h].k[j])).
+ * What lies behind len[r] in a page is not looked at, whatever it holds.  len[r] = 0: y is zero, lse -infinity; len[r] < 0: a place in a
+ * padded batch, whose row of y and lse stays as it is.  A length above max_len or the table is cut to it, a position whose page is not
+ * of the pool left out, a sequence that does not exist taken as empty; *status becomes THB_ERR_ARG.  max_len decides how a row is split among CTAs, and so the
+ * order of its sums; scratch is for the parts of one call at a time (thb_paged_attn_scratch bytes, 0: none is needed). */
+typedef struct thb_paged_attn_desc {
+    thb_kv_cache cache;
+    int rows, q_heads, q_ld, y_ld;
+    const int *len; /* [rows] */
+    const int *seq; /* [rows]; NULL: row r is sequence r */
+    int max_len;    /* no length is above it */
+    int window;     /* positions a token sees, itself among them; 0: all */
+    float scale;
+    float *lse;     /* [rows][q_heads]; NULL: not wanted */
+    void *scratch;
+    size_t scratch_bytes;
+} thb_paged_attn_desc;
+size_t thb_paged_attn_scratch(const thb_paged_attn_desc *d);
+int thb_paged_attn_fwd(const thb_paged_attn_desc *d, const void *q, void *y, thb_stream s);
+
 /* the launchers read their diagnostic THB200_* environment switches once; this re-reads them */
 void thb_conv_reload_knobs(void);
 const char *thb_last_cuda_error(void);

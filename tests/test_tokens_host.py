@@ -162,3 +162,45 @@ def test_rope_freq_host(lib):
         assert call(**bad)[0] == ARG, bad
     assert call(scaling=4)[0] == UNSUPPORTED and call(scaling=-1)[0] == UNSUPPORTED and call(dim=2, scaling=2)[0] == UNSUPPORTED
     assert call(dim=2)[0] == OK
+
+
+def attn_desc():
+    return K.PagedAttnDesc(cache=cache_desc(), rows=3, q_heads=8, q_ld=512, y_ld=520, len=AT, max_len=80, scale=0.1, scratch=AT, scratch_bytes=1 << 30)
+
+
+def test_paged_attn_refusals(lib):
+    def call(d, q=AT, y=AT):
+        return lib.thb_paged_attn_fwd(C.byref(d), q, y, None)
+
+    assert lib.thb_paged_attn_fwd(None, AT, AT, None) == ARG
+    for dtype in (K.THB_U8, 7):
+        assert call(changed(attn_desc, cache=cache_desc(dtype=dtype))) == UNSUPPORTED
+    for bad in BAD_CACHES:
+        assert call(changed(attn_desc, cache=cache_desc(**bad))) == ARG, bad
+    for bad in (dict(rows=-1), dict(q_heads=0), dict(q_heads=6), dict(q_heads=-4), dict(q_ld=504), dict(q_ld=516), dict(y_ld=256), dict(y_ld=514), dict(len=None),
+                dict(max_len=-1), dict(max_len=(1 << 30) + 1), dict(window=-1), dict(scale=float("inf")), dict(scale=float("nan")), dict(rows=4)):
+        assert call(changed(attn_desc, **bad)) == ARG, bad
+    for bad in (dict(q=None), dict(y=None), dict(q=AT + 8), dict(y=AT + 2)):
+        assert call(attn_desc(), **bad) == ARG, bad
+    assert call(changed(attn_desc, rows=0)) == OK
+    # a row of 80 positions is split: scratch is needed
+    need = lib.thb_paged_attn_scratch(C.byref(attn_desc()))
+    assert need > 0 and need % 4 == 0
+    for bad in (dict(scratch=None), dict(scratch_bytes=need - 1), dict(scratch=AT + 2)):
+        assert call(changed(attn_desc, **bad)) == ARG, bad
+    huge = cache_desc(heads=70000, token_stride=70000 * 64, page_stride=16 * 70000 * 64)
+    assert call(changed(attn_desc, cache=huge, q_heads=70000, q_ld=70000 * 64, y_ld=70000 * 64)) == UNSUPPORTED
+
+
+def test_paged_attn_scratch_covers_every_split(lib):
+    """The size grows with the rows, is none where nothing is split, and holds what a call's CTAs write at most."""
+    assert lib.thb_paged_attn_scratch(None) == 0
+    for rows in (1, 3, 100, 5000):
+        for max_len in (0, 1, 64, 65, 1000, 100000):
+            for window in (0, 40):
+                d = changed(attn_desc, rows=rows, max_len=max_len, window=window)
+                need = lib.thb_paged_attn_scratch(C.byref(d))
+                a_row = 8 * (64 + 2) * 4
+                span = min(max_len, window or max_len)
+                assert need % (rows * a_row) == 0 and need // (rows * a_row) <= max(1, (span + 63) // 64)
+                assert need == 0 or need // (rows * a_row) > 1

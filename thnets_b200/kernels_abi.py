@@ -84,6 +84,12 @@ class KvAppendDesc(C.Structure):
                 ("k_ld", C.c_int), ("v_ld", C.c_int), ("q_ld", C.c_int), ("q_out_ld", C.c_int), ("q_heads", C.c_int)]
 
 
+class PagedAttnDesc(C.Structure):
+    _fields_ = [("cache", KvCache), ("rows", C.c_int), ("q_heads", C.c_int), ("q_ld", C.c_int), ("y_ld", C.c_int),
+                ("len", C.c_void_p), ("seq", C.c_void_p), ("max_len", C.c_int), ("window", C.c_int), ("scale", C.c_float),
+                ("lse", C.c_void_p), ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t)]
+
+
 def aligned_tmap():
     """A 64-byte aligned thb_tmap plus the buffer that keeps it alive."""
     raw = (C.c_ubyte * (128 + 64))()
@@ -133,6 +139,9 @@ def load(libpath: str | None = None):
     lib.thb_q4_quantize_host.argtypes = [vp, cl, ci, cl, ci, ci, vp, ci, vp, ci, vp, ci]
     lib.thb_kv_append_fwd.argtypes = [C.POINTER(KvAppendDesc), vp, vp, vp, vp, vp]
     lib.thb_rope_freq_host.argtypes = [ci, C.c_double, ci, C.c_double, C.c_double, C.c_double, C.c_double, vp, C.POINTER(cf)]
+    lib.thb_paged_attn_scratch.argtypes = [C.POINTER(PagedAttnDesc)]
+    lib.thb_paged_attn_scratch.restype = C.c_size_t
+    lib.thb_paged_attn_fwd.argtypes = [C.POINTER(PagedAttnDesc), vp, vp, vp]
     lib.thb_last_cuda_error.restype = C.c_char_p
     lib.thb_kernel_launch_count.restype = ci
     return lib
