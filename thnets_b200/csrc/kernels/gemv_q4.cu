@@ -39,59 +39,88 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// codes i and i + 4 of a word (nibbles, lowest first) less the zero point, as a pair of 16-bit numbers; zp = (zero + base) twice
-template <bool BF> __device__ __forceinline__ uint32_t pair_of(uint32_t word, int i, uint32_t zp)
+// (a & mask) | base in one instruction
+__device__ __forceinline__ uint32_t code_pair(uint32_t a, uint32_t mask, uint32_t base)
 {
-    uint32_t v = word >> (4 * i);
-    if (BF) {
-        v = (v & 0x000f000fu) | 0x43004300u;
-        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&v), *reinterpret_cast<const __nv_bfloat162 *>(&zp));
-        return *reinterpret_cast<const uint32_t *>(&d);
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(base));
+    return d;
+}
+// the zero point of a row's group as what is subtracted from a pair: z + 1024 (fp16) or z + 128 (bf16) twice
+template <bool BF> __device__ __forceinline__ uint32_t zero_pair(uint32_t z) { return ((z & 15) | (BF ? 0x4300u : 0x6400u)) * 0x10001u; }
+// codes (0, 4), (1, 5), (2, 6), (3, 7) of a word (nibbles, lowest first) less the zero point, as pairs of 16-bit numbers.  In fp16 the odd
+// ones are taken where they stand, as 1024 + 16 q, and scaled by the subtraction of 64 + z.
+template <bool BF> __device__ __forceinline__ void pairs_of(uint32_t word, uint32_t za, uint32_t zb, uint32_t (&d)[4])
+{
+    if constexpr (BF) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t v = code_pair(word >> (4 * i), 0x000f000fu, 0x43004300u);
+            const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v), *reinterpret_cast<const __nv_bfloat162 *>(&za));
+            d[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const uint32_t u = i ? word >> 8 : word, v = code_pair(u, 0x000f000fu, 0x64006400u), w = code_pair(u, 0x00f000f0u, 0x64006400u);
+            const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&za));
+            const __half2 k = __hfma2(*reinterpret_cast<const __half2 *>(&w), __float2half2_rn(0.0625f), *reinterpret_cast<const __half2 *>(&zb));
+            d[i] = *reinterpret_cast<const uint32_t *>(&h);
+            d[i + 1] = *reinterpret_cast<const uint32_t *>(&k);
+        }
     }
-    v = (v & 0x000f000fu) | 0x64006400u;
-    const __half2 d = __hsub2(*reinterpret_cast<__half2 *>(&v), *reinterpret_cast<const __half2 *>(&zp));
+}
+// -(64 + z) from 1024 + z
+__device__ __forceinline__ uint32_t zero_pair_16(uint32_t za)
+{
+    const __half2 d = __hsub2(__float2half2_rn(960.f), *reinterpret_cast<const __half2 *>(&za));
     return *reinterpret_cast<const uint32_t *>(&d);
 }
 
-// 8 consecutive values of x from k on as four B registers a part: (x0,x4), (x1,x5), (x2,x6), (x3,x7); zeros from K on
-template <typename X> struct XLoad;
-template <bool BF16> struct XLoad16 {
-    static __device__ __forceinline__ void get(const void *x, long row, int k, int K, uint32_t (&b)[1][4])
+// What a lane holds of 8 consecutive values of its row of x, as loaded and as four B registers a part: (x0,x4), (x1,x5), (x2,x6), (x3,x7)
+template <typename X> struct XVec;
+struct XVec16 {
+    uint4 v;
+    __device__ __forceinline__ void load(const void *x, long row, int k, int K)
     {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (k < K) {
-            v = *reinterpret_cast<const uint4 *>((const uint16_t *)x + row + k);
-            if (k + 8 > K) {
-                uint32_t *h = reinterpret_cast<uint32_t *>(&v);
+        v = make_uint4(0, 0, 0, 0);
+        if (k < K) v = *reinterpret_cast<const uint4 *>((const uint16_t *)x + row + k);
+    }
+    __device__ __forceinline__ void cut(int left)  // values from `left` on (0 < left < 8) lie behind the row
+    {
+        uint32_t *h = reinterpret_cast<uint32_t *>(&v);
 #pragma unroll
-                for (int i = 0; i < 4; i++) h[i] &= k + 2 * i + 1 < K ? 0xffffffffu : k + 2 * i < K ? 0xffffu : 0u;
-            }
-        }
+        for (int i = 0; i < 4; i++) h[i] &= 2 * i + 1 < left ? 0xffffffffu : 2 * i < left ? 0xffffu : 0u;
+    }
+    __device__ __forceinline__ void get(uint32_t (&b)[1][4]) const
+    {
         b[0][0] = __byte_perm(v.x, v.z, 0x5410);
         b[0][1] = __byte_perm(v.x, v.z, 0x7632);
         b[0][2] = __byte_perm(v.y, v.w, 0x5410);
         b[0][3] = __byte_perm(v.y, v.w, 0x7632);
     }
 };
-template <> struct XLoad<XF16> : XLoad16<false> {};
-template <> struct XLoad<XBF16> : XLoad16<true> {};
-template <> struct XLoad<XE4M3> {
+template <> struct XVec<XF16> : XVec16 {};
+template <> struct XVec<XBF16> : XVec16 {};
+template <> struct XVec<XE4M3> {
+    uint2 v;
     static __device__ __forceinline__ uint32_t two(uint32_t codes)  // two codes in the low halfword -> two fp16
     {
         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
         return (uint32_t)h.x | (uint32_t)h.y << 16;
     }
-    static __device__ __forceinline__ void get(const void *x, long row, int k, int K, uint32_t (&b)[1][4])
+    __device__ __forceinline__ void load(const void *x, long row, int k, int K)
     {
-        uint2 v = make_uint2(0, 0);
-        if (k < K) {
-            v = *reinterpret_cast<const uint2 *>((const uint8_t *)x + row + k);
-            const int left = K - k;
-            if (left < 8) {
-                v.x &= left >= 4 ? 0xffffffffu : (1u << 8 * left) - 1;
-                v.y &= left <= 4 ? 0u : (1u << 8 * (left - 4)) - 1;
-            }
-        }
+        v = make_uint2(0, 0);
+        if (k < K) v = *reinterpret_cast<const uint2 *>((const uint8_t *)x + row + k);
+    }
+    __device__ __forceinline__ void cut(int left)
+    {
+        v.x &= left >= 4 ? 0xffffffffu : (1u << 8 * left) - 1;
+        v.y &= left <= 4 ? 0u : (1u << 8 * (left - 4)) - 1;
+    }
+    __device__ __forceinline__ void get(uint32_t (&b)[1][4]) const
+    {
         const uint32_t p = __byte_perm(v.x, v.y, 0x5140), r = __byte_perm(v.x, v.y, 0x7362);  // codes 0 4 1 5 and 2 6 3 7
         b[0][0] = two(p);
         b[0][1] = two(p >> 16);
@@ -99,34 +128,35 @@ template <> struct XLoad<XE4M3> {
         b[0][3] = two(r >> 16);
     }
 };
-template <> struct XLoad<XF32> {
-    static __device__ __forceinline__ void get(const void *x, long row, int k, int K, uint32_t (&b)[3][4])
+template <> struct XVec<XF32> {
+    float v[8];
+    __device__ __forceinline__ void load(const void *x, long row, int k, int K)
     {
-        float v[8];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-            const int at = k + 4 * h;
-            if (at < K) {
-                f = *reinterpret_cast<const float4 *>((const float *)x + row + at);
-                if (at + 1 >= K) f.y = 0.f;
-                if (at + 2 >= K) f.z = 0.f;
-                if (at + 3 >= K) f.w = 0.f;
-            }
+            if (k + 4 * h < K) f = *reinterpret_cast<const float4 *>((const float *)x + row + k + 4 * h);
             v[4 * h] = f.x; v[4 * h + 1] = f.y; v[4 * h + 2] = f.z; v[4 * h + 3] = f.w;
         }
-        // a part is the top 16 bits of what the parts before it leave: 8 bits of mantissa each, no rounding, the rest is exact.
-        // (infinities and NaN: the first part is the value, the others must not turn an infinity into NaN)
+    }
+    __device__ __forceinline__ void cut(int left)
+    {
+#pragma unroll
+        for (int i = 1; i < 8; i++) v[i] = i < left ? v[i] : 0.f;
+    }
+    // A part is the top 16 bits of what the parts before it leave: 8 bits of mantissa each, no rounding, the rest is exact (that of an
+    // infinity is zero, not NaN).
+    __device__ __forceinline__ void get(uint32_t (&b)[3][4]) const
+    {
         uint32_t part[3][8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const uint32_t u = __float_as_uint(v[i]);
-            const bool fin = (u & 0x7f800000u) != 0x7f800000u;
-            part[0][i] = fin || !(u & 0x7fffffu) ? u : 0x7fc00000u;
-            const float r1 = v[i] - __uint_as_float(u & 0xffff0000u);
-            part[1][i] = fin ? __float_as_uint(r1) : 0u;
-            const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
-            part[2][i] = fin ? __float_as_uint(r2) : 0u;
+            part[0][i] = __float_as_uint(v[i]);
+#pragma unroll
+            for (int q = 1; q < 3; q++) {
+                const float x = __uint_as_float(part[q - 1][i]), top = __uint_as_float(part[q - 1][i] & 0xffff0000u);
+                part[q][i] = __float_as_uint(x == top ? 0.f : x - top);
+            }
         }
 #pragma unroll
         for (int q = 0; q < 3; q++)
@@ -135,142 +165,334 @@ template <> struct XLoad<XF32> {
     }
 };
 
-__device__ __forceinline__ float wscale_at(const void *s, int dtype, long i)
+__device__ __forceinline__ float scale_of(uint32_t bits, int dtype)
 {
-    if (dtype == THB_F32) return ((const float *)s)[i];
-    if (dtype == THB_F16) return __half2float(((const __half *)s)[i]);
-    return __bfloat162float(((const __nv_bfloat16 *)s)[i]);
+    if (dtype == THB_F32) return __uint_as_float(bits);
+    return dtype == THB_F16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
 }
 
-// A CTA takes 16 rows of weights, its eight warps an eighth of the blocks of 128 k each, in order; the parts are added at the end.
-// Lane (g = lane / 4, t = lane % 4) holds rows g and g + 8.  Of a block it loads the k of its t: 32 in one vector where a group is 128
-// long, 16 of each of two groups, 8 of each of four, so that a product's k are all of one group.
-template <typename X, int GROUP>
-__global__ void __launch_bounds__(256) gemv_q4_kernel(Q4Params p)
-{
-    constexpr int AHEAD = 4;                  // blocks under way a warp
-    constexpr int VW = GROUP / 32, NG = 128 / GROUP;  // words a load, groups a block
-    __shared__ float part[8][128];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int m0 = blockIdx.x * 16;
-    const int blocks = (p.K + 127) / 128, groups = (p.K + GROUP - 1) / GROUP, bytes = ((p.K + 1) / 2 + 15) / 16 * 16;
-    const int b0 = blocks * warp / 8, b1 = blocks * (warp + 1) / 8;
-    // (rows beyond the last are read as the last and not written)
-    const long row[2] = {min(m0 + g, p.M - 1), min(m0 + g + 8, p.M - 1)};
+// How a launch is cut, by the shape alone: the warps of a CTA are wk along k times WARPS / wk tiles of 16 rows; a row's blocks of 128 k are
+// walked in `chunks` passes of wk warps by `mine` blocks each.
+struct Q4Cut {
+    int wk, mine, chunks, tiles, wide;  // wide: scales and zero points are aligned to what a lane loads of them
+};
+#ifndef Q4W
+#define Q4W 8
+#endif
+constexpr int WARPS = Q4W, Q4_ACC = 64;  // warps a CTA; tiles whose sums a CTA keeps between chunks
+constexpr int COL = 20, PITCH = 8 * COL;  // floats a column, and a warp's part, take in shared memory: no bank twice in the parts' writes
 
-    uint32_t w[AHEAD][2][4];
-    float s[AHEAD][2][NG];
-    uint32_t z[AHEAD][2][NG];
-    auto load = [&](int slot, int b) {
+template <typename X> struct Q4Shape {
+    static constexpr int NB = (X::PARTS == 3 ? 16 : 32) / WARPS;  // blocks a stage at most
+    static constexpr int STAGES = X::PARTS == 3 ? 8 : 4;
+    static constexpr int RING = WARPS * STAGES * NB * 1024, FIXED = RING + 2 * WARPS * PITCH * 4;
+};
+
+// One CTA to an SM owns a range of tiles.  A warp keeps its part of x in registers as B operands and walks the CTA's
+// tiles past it; the codes come through a ring of its own in shared memory, 16 rows by `mine` blocks a stage, by cp.async of 16 bytes (no
+// registers and no barrier between warps: up to 128 KB under way an SM).  The warps' parts are added at a tile's end; where a row has
+// more chunks than one, the sums stay in shared memory until the last, and x of the next chunk is loaded during the last tile of this one.
+// Lane (g = lane / 4, t = lane % 4) holds rows g and g + 8.  Of a block it takes the k of its t: 32 in one vector where a group is 128
+// long, 16 of each of two groups, 8 of each of four, so that a product's k are all of one group.
+template <typename X, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cut cut)
+{
+    constexpr int NB = Q4Shape<X>::NB, STAGES = Q4Shape<X>::STAGES;
+    constexpr int VW = GROUP / 32, NG = 128 / GROUP;             // words a load, groups a block
+    constexpr int GL = NB * NG > 4 ? NB * NG / 4 : 1;            // groups whose scale a lane loads
+    constexpr int RS = 32 / (NB * 4);                            // rows a warp's cp.async covers (NB = 1: 8, 2: 4, 4: 2)
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    float *part = reinterpret_cast<float *>(smem + Q4Shape<X>::RING);  // [2][warps][PITCH]
+    float *sums = part + 2 * WARPS * PITCH;                            // [tiles of the CTA][128], where there are chunks
+    const uint32_t ring = smem_u32(smem) + warp * STAGES * NB * 1024;
+
+    const int tile0 = (int)((long)cut.tiles * blockIdx.x / gridDim.x), tile1 = (int)((long)cut.tiles * (blockIdx.x + 1) / gridDim.x);
+    const int wk = cut.wk, wm = WARPS / wk, kw = warp % wk, mw = warp / wk;
+    const int steps = (tile1 - tile0 + wm - 1) / wm;
+    const int groups = (p.K + GROUP - 1) / GROUP, bytes = ((p.K + 1) / 2 + 15) / 16 * 16;
+
+    // 16-byte pieces of a stage, permuted so that no load of 8, 4 or 2 rows meets a bank twice (rows of 64 bytes lie two to a line)
+    auto piece = [](int row, int c) {
+        const int at = row * (NB * 4) + c, line = at >> 3;
+        const int f = VW == 4 ? (NB >= 2 ? (row & 1) << 2 : 0) : VW == 2 ? (NB >= 2 ? (row & 3) << 1 : (line & 1) << 1) : (NB >= 2 ? row & 7 : line & 3);
+        return (at ^ f) * 16;
+    };
+
+    // ---- the codes' loads, STAGES - 1 units (a tile of a chunk) ahead
+    int ftile = tile0 + mw, fchunk = 0, fslot = 0;
+    const int fr = lane / (NB * 4), fc = lane % (NB * 4);
+    const uint8_t *fsrc = p.w;
+    long fstep = 0, fnext = 0;
+    uint32_t fsize = 0;
+    auto seek = [&] {
+        const int o = (fchunk * wk + kw) * cut.mine * 64 + fc * 16;
+        const bool in = fchunk < cut.chunks && fc < cut.mine * 4 && o < bytes;
+        fsize = in ? 16 : 0;
+        fsrc = in ? p.w + (long)(ftile * 16 + fr) * p.w_ld + o : p.w;
+        fstep = in ? (long)RS * p.w_ld : 0;
+        fnext = in ? (long)(wm - 1) * 16 * p.w_ld : 0;
+    };
+    seek();
+    auto fetch = [&] {
+        const uint32_t at = ring + fslot * (NB * 1024);
+        if (ftile < tile1 && ftile * 16 + 16 <= p.M) {
+#pragma unroll
+            for (int i = 0; i < 16 / RS; i++) {
+                cp_async16(at + piece(i * RS + fr, fc), fsrc, fsize);
+                fsrc += fstep;
+            }
+        } else {  // (rows beyond the last are zeros and not written)
+#pragma unroll
+            for (int i = 0; i < 16 / RS; i++) {
+                const bool in = ftile < tile1 && ftile * 16 + i * RS + fr < p.M;
+                cp_async16(at + piece(i * RS + fr, fc), in ? fsrc : p.w, in ? fsize : 0);
+                fsrc += fstep;
+            }
+        }
+        fsrc += fnext;
+        cp_async_commit();
+        fslot = fslot + 1 == STAGES ? 0 : fslot + 1;
+        ftile += wm;
+        if (ftile - mw >= tile0 + steps * wm) {
+            ftile = tile0 + mw;
+            fchunk++;
+            seek();
+        }
+    };
+    // ---- the scales and zero points of a unit, one unit ahead, as they lie in memory (`wide`: 16-bit scales two to a word, zero points four);
+    // a lane loads those of GL groups of rows g and g + 8
+    uint32_t sn[2][GL], zn[2][GL];
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+        for (int i = 0; i < GL; i++) sn[r][i] = zn[r][i] = 0;
+    auto fetch_scales = [&](int chunk, int tile) {
+        const int j = t % (NB * NG / GL) * GL, group = (chunk * wk + kw) * cut.mine * NG + j;
+        if (chunk >= cut.chunks || tile >= tile1 || j >= cut.mine * NG) return;
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-            const uint8_t *at = p.w + row[r] * p.w_ld;
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                const int o = b * 64 + j * (GROUP / 2) + t * 4 * VW;
-                uint32_t *d = w[slot][r] + j * VW;
-#pragma unroll
-                for (int i = 0; i < VW; i++) d[i] = 0;
-                s[slot][r][j] = 0.f;
-                z[slot][r][j] = 8;
-                if (b < b1 && o < bytes) {
-                    if (VW == 4) {
-                        const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(at + o));
-                        d[0] = v.x; d[1 % VW] = v.y; d[2 % VW] = v.z; d[3 % VW] = v.w;
-                    } else if (VW == 2) {
-                        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(at + o));
-                        d[0] = v.x; d[1 % VW] = v.y;
-                    } else
-                        d[0] = __ldg(reinterpret_cast<const uint32_t *>(at + o));
+            const long row = tile * 16 + r * 8 + g;
+            if (row >= p.M) continue;
+            const long at = row * p.s_ld + group;
+            if (cut.wide && GL > 1) {
+                if (group < groups) {
+                    if (GL == 2) sn[r][0] = __ldg(reinterpret_cast<const uint32_t *>((const unsigned short *)p.wscale + at));
+                    else {
+                        const uint2 v = __ldg(reinterpret_cast<const uint2 *>((const unsigned short *)p.wscale + at));
+                        sn[r][0] = v.x;
+                        sn[r][GL > 1] = v.y;
+                    }
                 }
-                const int group = b * NG + j;
-                if (b < b1 && group < groups) {
-                    s[slot][r][j] = wscale_at(p.wscale, p.s_dtype, row[r] * p.s_ld + group);
-                    if (p.wzero) z[slot][r][j] = p.wzero[row[r] * p.z_ld + group];
+            } else {
+#pragma unroll
+                for (int i = 0; i < GL; i++)
+                    if (group + i < groups) sn[r][i] = p.s_dtype == THB_F32 ? __ldg((const uint32_t *)p.wscale + at + i) : __ldg((const unsigned short *)p.wscale + at + i);
+            }
+            if (ZEROS) {
+                const uint8_t *z = p.wzero + row * p.z_ld + group;
+                if (cut.wide && GL == 4) {
+                    if (group < groups) zn[r][0] = __ldg(reinterpret_cast<const uint32_t *>(z));
+                } else if (cut.wide && GL == 2) {
+                    if (group < groups) zn[r][0] = __ldg(reinterpret_cast<const unsigned short *>(z));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < GL; i++)
+                        if (group + i < groups) zn[r][i] = __ldg(z + i);
                 }
             }
         }
     };
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+
+    // ---- x of a chunk: as loaded, and as operands
     const long xrow = (long)(g < p.N ? g : 0) * p.x_ld;
     const int xk = g < p.N ? p.K : 0;  // (columns beyond the rows of x are zeros)
-    auto consume = [&](int slot, int b) {
+    XVec<X> raw[NB][4];
+    uint32_t xb[NB][4][X::PARTS][4];
+    auto x_at = [&](int chunk, int n, int i) { return ((chunk * wk + kw) * cut.mine + n) * 128 + (i / VW) * GROUP + t * 8 * VW + (i % VW) * 8; };
+    auto load_x = [&](int chunk) {
 #pragma unroll
-        for (int j = 0; j < NG; j++) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            uint32_t zp[2];
+        for (int n = 0; n < NB; n++)
 #pragma unroll
-            for (int r = 0; r < 2; r++) zp[r] = ((z[slot][r][j] & 15) | (X::BF ? 0x4300u : 0x6400u)) * 0x10001u;
+            for (int i = 0; i < 4; i++) raw[n][i].load(p.x, xrow, x_at(chunk, n, i), n < cut.mine ? xk : 0);
+    };
+    auto take_x = [&](int chunk) {
 #pragma unroll
-            for (int i = 0; i < VW; i++) {
-                uint32_t xb[X::PARTS][4];
-                XLoad<X>::get(p.x, xrow, b * 128 + j * GROUP + t * 8 * VW + i * 8, xk, xb);
-                uint32_t a[2][4];
+        for (int n = 0; n < NB; n++)
 #pragma unroll
-                for (int r = 0; r < 2; r++)
+            for (int i = 0; i < 4; i++) {
+                const int left = p.K - x_at(chunk, n, i);
+                if (left > 0 && left < 8) raw[n][i].cut(left);
+                raw[n][i].get(xb[n][i]);
+            }
+    };
+
+    // The weights do not depend on the launch before this one: the first stages are under way while that one drains.
+#pragma unroll 1
+    for (int u = 0; u < STAGES - 1; u++) fetch();
+    fetch_scales(0, tile0 + mw);
+    pdl_enter();
+    load_x(0);
+
+    // where this lane's codes of row g lie in a stage: pieces differ in bits 4 to 6 by what their number differs in, then by whole lines
+    const uint32_t mine_at = warp * STAGES * NB * 1024 + piece(g, t * VW / 4) + t * VW % 4 * 4;
+    int slot = 0, parity = 0;
+    for (int chunk = 0; chunk < cut.chunks; chunk++) {
+        take_x(chunk);
+        for (int step = 0; step < steps; step++) {
+            float sv[2][GL];
+            uint32_t zv[2][GL];
 #pragma unroll
-                    for (int q = 0; q < 4; q++) a[r][q] = pair_of<X::BF>(w[slot][r][j * VW + i], q, zp[r]);
+            for (int r = 0; r < 2; r++)
 #pragma unroll
-                for (int q = X::PARTS - 1; q >= 0; q--) {
-                    mma16816<X::BF>(c, a[0][0], a[1][0], a[0][1], a[1][1], xb[q][0], xb[q][1]);
-                    mma16816<X::BF>(c, a[0][2], a[1][2], a[0][3], a[1][3], xb[q][2], xb[q][3]);
+                for (int i = 0; i < GL; i++) {
+                    const bool packed = cut.wide && GL > 1;
+                    const uint32_t bits = packed ? sn[r][i / 2] >> (16 * (i & 1)) : sn[r][i];
+                    sv[r][i] = scale_of(bits, p.s_dtype);
+                    if (ZEROS) zv[r][i] = zero_pair<X::BF>(packed ? zn[r][0] >> (8 * i) : zn[r][i]);
+                }
+            // what lies behind a row's groups is not a scale (rows behind the last have any, and are not written)
+            if (((chunk * wk + kw) + 1) * cut.mine * NG > groups) {
+                const int group = (chunk * wk + kw) * cut.mine * NG + t % (NB * NG / GL) * GL;
+#pragma unroll
+                for (int i = 0; i < GL; i++)
+                    if (group + i >= groups) sv[0][i] = sv[1][i] = 0.f;
+            }
+            cp_async_wait<STAGES - 2>();
+            __syncwarp();
+            fetch();
+            const bool last = step == steps - 1;
+            fetch_scales(last ? chunk + 1 : chunk, tile0 + mw + (last ? 0 : (step + 1) * wm));
+            if (last && chunk + 1 < cut.chunks) load_x(chunk + 1);
+
+            const uint32_t at = mine_at + slot * (NB * 1024);
+            slot = slot + 1 == STAGES ? 0 : slot + 1;
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                if (n >= cut.mine) break;
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t w[2][VW], za[2], zb[2];
+                    float sc[2];
+                    constexpr int LINE = NB >= 2 ? 8 : 4;  // pieces of a row in a line
+                    const int c0 = n * 4 + j * (GROUP / 32);
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const uint8_t *src = smem + (at ^ c0 % LINE * 16) + c0 / LINE * 128 + r * (8 * NB * 64);
+                        if constexpr (VW == 4) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(src);
+                            w[r][0] = v.x; w[r][1 % VW] = v.y; w[r][2 % VW] = v.z; w[r][3 % VW] = v.w;
+                        } else if constexpr (VW == 2) {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(src);
+                            w[r][0] = v.x; w[r][1 % VW] = v.y;
+                        } else
+                            w[r][0] = *reinterpret_cast<const uint32_t *>(src);
+                        const int group = n * NG + j, from = (lane & ~3) | group / GL;
+                        sc[r] = __shfl_sync(0xffffffffu, sv[r][group % GL], from);
+                        za[r] = ZEROS ? __shfl_sync(0xffffffffu, zv[r][group % GL], from) : zero_pair<X::BF>(8);
+                        zb[r] = X::BF ? 0 : zero_pair_16(za[r]);
+                    }
+#pragma unroll
+                    for (int h = 0; h < VW; h++) {
+                        uint32_t a[2][4];
+#pragma unroll
+                        for (int r = 0; r < 2; r++) pairs_of<X::BF>(w[r][h], za[r], zb[r], a[r]);
+#pragma unroll
+                        for (int q = X::PARTS - 1; q >= 0; q--) {
+                            const uint32_t(&b)[4] = xb[n][j * VW + h][q];
+                            mma16816<X::BF>(c, a[0][0], a[1][0], a[0][1], a[1][1], b[0], b[1]);
+                            mma16816<X::BF>(c, a[0][2], a[1][2], a[0][3], a[1][3], b[2], b[3]);
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; q++) acc[q] = fmaf(c[q], sc[q >> 1], acc[q]);
                 }
             }
-            acc[0] = fmaf(c[0], s[slot][0][j], acc[0]);
-            acc[1] = fmaf(c[1], s[slot][0][j], acc[1]);
-            acc[2] = fmaf(c[2], s[slot][1][j], acc[2]);
-            acc[3] = fmaf(c[3], s[slot][1][j], acc[3]);
-        }
-    };
-    // The weights do not depend on the launch before this one: the first blocks are under way while that one drains.
+            // the tile's parts.  c0, c1: row g, columns 2t and 2t + 1; c2, c3: row g + 8
+            float *const parts = part + parity * WARPS * PITCH;
 #pragma unroll
-    for (int i = 0; i < AHEAD; i++) load(i, b0 + i);
-    pdl_enter();
-    for (int b = b0; b < b1; b += AHEAD) {
-#pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            if (b + i >= b1) break;
-            consume(i, b + i);
-            load(i, b + i + AHEAD);
-        }
-    }
-    // c0, c1: row g, columns 2t and 2t + 1; c2, c3: row g + 8
-#pragma unroll
-    for (int i = 0; i < 4; i++) part[warp][(2 * t + (i & 1)) * 16 + g + (i >> 1) * 8] = acc[i];
-    __syncthreads();
-    if (tid < 128) {
-        const int n = tid >> 4, m = m0 + (tid & 15);
-        const int al = p.dtype == THB_F32 ? 4 : 8;
-        if (n < p.N && m < p.M) {
-            float v = 0.f;
-#pragma unroll
-            for (int q = 0; q < 8; q++) v += part[q][tid];
-            if (p.x_scale) v *= p.x_scale[n];
-            const float sc = p.scale ? p.scale[m] : 1.f, sh = p.shift ? p.shift[m] : 0.f;
-            const float sl = p.act.kind == THB_ACT_PRELU ? p.act.slope[m] : 0.f;
-            v = thb_apply_act(v * sc + sh, p.act.kind, p.act.threshold, p.act.value, p.act.alpha, sl);
-            const long o = (long)n * p.y_ld + m;
-            if (p.dtype == THB_F32) ((float *)p.y)[o] = v;
-            else if (p.dtype == THB_F16) ((__half *)p.y)[o] = __float2half_rn(v);
-            else ((__nv_bfloat16 *)p.y)[o] = __float2bfloat16_rn(v);
-        } else if (n < p.N && m < (p.M + al - 1) / al * al) {
-            // channels of the padded tail of y are kept at exact zero
-            const long o = (long)n * p.y_ld + m;
-            if (p.dtype == THB_F32) ((float *)p.y)[o] = 0.f;
-            else ((uint16_t *)p.y)[o] = 0;
+            for (int q = 0; q < 4; q++) parts[warp * PITCH + (2 * t + (q & 1)) * COL + g + (q >> 1) * 8] = acc[q];
+            __syncthreads();  // (the buffers alternate, so that one barrier a step is enough)
+            parity ^= 1;
+            // four warps add a tile's parts, two columns each, and the steps go round the warps
+            for (int i = 0; i < wm; i++) {
+                const int turn = (step * wm + i) % (WARPS / 4), local = step * wm + i, tile = tile0 + local;
+                const int n = (warp & 3) * 2 + (lane >> 4), row = lane & 15, m = tile * 16 + row;
+                if (warp / 4 != turn || n >= p.N || tile >= tile1) continue;
+                const float *from = parts + i * wk * PITCH + n * COL + row;
+                float v = 0.f;
+                for (int q = 0; q < wk; q++) v += from[q * PITCH];
+                float *sum = sums + local * 128 + n * 16 + row;
+                if (chunk > 0) v += *sum;
+                if (chunk + 1 < cut.chunks) {
+                    *sum = v;  // (the same thread comes for it)
+                    continue;
+                }
+                if (m >= (p.M + 7) / 8 * 8 || (p.dtype == THB_F32 && m >= (p.M + 3) / 4 * 4)) continue;
+                if (m < p.M) {
+                    if (p.x_scale) v *= p.x_scale[n];
+                    if (p.scale) v *= p.scale[m];
+                    if (p.shift) v += p.shift[m];
+                    if (p.act.kind != THB_ACT_NONE)
+                        v = thb_apply_act(v, p.act.kind, p.act.threshold, p.act.value, p.act.alpha, p.act.kind == THB_ACT_PRELU ? p.act.slope[m] : 0.f);
+                } else
+                    v = 0.f;  // channels of the padded tail of y are kept at exact zero
+                const long to = (long)n * p.y_ld + m;
+                if (p.dtype == THB_F32) ((float *)p.y)[to] = v;
+                else if (p.dtype == THB_F16) ((__half *)p.y)[to] = __float2half_rn(v);
+                else ((__nv_bfloat16 *)p.y)[to] = __float2bfloat16_rn(v);
+            }
         }
     }
+    cp_async_wait<0>();
+}
+
+template <typename X, int GROUP, bool ZEROS> int launch_q4_group(const Q4Params &p, cudaStream_t st)
+{
+    constexpr int NB = Q4Shape<X>::NB, FIXED = Q4Shape<X>::FIXED;
+    constexpr int GL = NB * (128 / GROUP) > 4 ? NB * (128 / GROUP) / 4 : 1;
+    const auto kern = gemv_q4_kernel<X, GROUP, ZEROS>;
+    static int sms[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return thb_refuse(THB_ERR_UNSUPPORTED, "thb_gemv_q4_fwd: device ordinal above 63");
+    if (!sms[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FIXED + Q4_ACC * 512);
+        if (e != cudaSuccess) return thb_note_launch(e, "gemv_q4_kernel attributes");
+        sms[dev] = thb_sm_count();
+    }
+    Q4Cut c;
+    const int blocks = (p.K + 127) / 128;
+    c.tiles = (p.M + 15) / 16;
+    c.wk = WARPS;
+    while (c.wk > 1 && c.wk / 2 * NB >= blocks) c.wk /= 2;
+    c.chunks = (blocks + c.wk * NB - 1) / (c.wk * NB);
+    c.mine = (blocks + c.wk * c.chunks - 1) / (c.wk * c.chunks);
+    c.wide = p.s_dtype != THB_F32 && p.s_ld % GL == 0 && reinterpret_cast<uintptr_t>(p.wscale) % (2 * GL) == 0 && (!p.wzero || (p.z_ld % GL == 0 && reinterpret_cast<uintptr_t>(p.wzero) % GL == 0));
+    int grid = c.tiles < sms[dev] ? c.tiles : sms[dev];
+    if (c.chunks > 1 && grid < (c.tiles + Q4_ACC - 1) / Q4_ACC) grid = (c.tiles + Q4_ACC - 1) / Q4_ACC;
+    const int most = (c.tiles + grid - 1) / grid;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = FIXED + (c.chunks > 1 ? most * 512 : 0);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = thb_pdl_enabled() ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, c);
+    return thb_note_launch(e != cudaSuccess ? e : cudaGetLastError(), "gemv_q4_kernel");
 }
 
 template <typename X> int launch_q4(const Q4Params &p, int group, cudaStream_t st)
 {
-    const unsigned grid = (p.M + 15) / 16;
-    switch (group) {
-    case 32: thb_launch(gemv_q4_kernel<X, 32>, grid, 256, st, p); break;
-    case 64: thb_launch(gemv_q4_kernel<X, 64>, grid, 256, st, p); break;
-    default: thb_launch(gemv_q4_kernel<X, 128>, grid, 256, st, p);
-    }
-    return THB_LAUNCH_CHECK("gemv_q4_kernel");
+    if (group == 32) return p.wzero ? launch_q4_group<X, 32, true>(p, st) : launch_q4_group<X, 32, false>(p, st);
+    if (group == 64) return p.wzero ? launch_q4_group<X, 64, true>(p, st) : launch_q4_group<X, 64, false>(p, st);
+    return p.wzero ? launch_q4_group<X, 128, true>(p, st) : launch_q4_group<X, 128, false>(p, st);
 }
 
 }  // namespace
