@@ -32,10 +32,10 @@ template <bool BF>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
     if (BF)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
@@ -165,27 +165,23 @@ template <> struct XVec<XF32> {
     }
 };
 
-__device__ __forceinline__ float scale_of(uint32_t bits, int dtype)
-{
-    if (dtype == THB_F32) return __uint_as_float(bits);
-    return dtype == THB_F16 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
-}
-
 // How a launch is cut, by the shape alone: the warps of a CTA are wk along k times WARPS / wk tiles of 16 rows; a row's blocks of 128 k are
 // walked in `chunks` passes of wk warps by `mine` blocks each.
 struct Q4Cut {
-    int wk, mine, chunks, tiles, wide;  // wide: scales and zero points are aligned to what a lane loads of them
+    int wk, mine, chunks, tiles, wide;  // wide: 16-bit scales, and zero points, are aligned to what a lane loads of them
 };
 #ifndef Q4W
 #define Q4W 8
 #endif
+static_assert(Q4W == 8, "two groups of four warps");
 constexpr int WARPS = Q4W, Q4_ACC = 64;  // warps a CTA; tiles whose sums a CTA keeps between chunks
 constexpr int COL = 20, PITCH = 8 * COL;  // floats a column, and a warp's part, take in shared memory: no bank twice in the parts' writes
 
 template <typename X> struct Q4Shape {
     static constexpr int NB = (X::PARTS == 3 ? 16 : 32) / WARPS;  // blocks a stage at most
     static constexpr int STAGES = X::PARTS == 3 ? 8 : 4;
-    static constexpr int RING = WARPS * STAGES * NB * 1024, FIXED = RING + 2 * WARPS * PITCH * 4;
+    static constexpr int SCALES = 2 * 16 * (NB * 4 + 4) * 4;      // bytes of scales and zero points a warp
+    static constexpr int RING = WARPS * STAGES * NB * 1024, FIXED = RING + 2 * WARPS * PITCH * 4 + WARPS * SCALES;
 };
 
 // One CTA to an SM owns a range of tiles.  A warp keeps its part of x in registers as B operands and walks the CTA's
@@ -199,12 +195,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
 {
     constexpr int NB = Q4Shape<X>::NB, STAGES = Q4Shape<X>::STAGES;
     constexpr int VW = GROUP / 32, NG = 128 / GROUP;             // words a load, groups a block
-    constexpr int GL = NB * NG > 4 ? NB * NG / 4 : 1;            // groups whose scale a lane loads
     constexpr int RS = 32 / (NB * 4);                            // rows a warp's cp.async covers (NB = 1: 8, 2: 4, 4: 2)
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     float *part = reinterpret_cast<float *>(smem + Q4Shape<X>::RING);  // [2][warps][PITCH]
-    float *sums = part + 2 * WARPS * PITCH;                            // [tiles of the CTA][128], where there are chunks
+    float *sums = reinterpret_cast<float *>(smem + Q4Shape<X>::FIXED);  // [tiles of the CTA][128], where there are chunks
     const uint32_t ring = smem_u32(smem) + warp * STAGES * NB * 1024;
 
     const int tile0 = (int)((long)cut.tiles * blockIdx.x / gridDim.x), tile1 = (int)((long)cut.tiles * (blockIdx.x + 1) / gridDim.x);
@@ -260,48 +255,77 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
             seek();
         }
     };
-    // ---- the scales and zero points of a unit, one unit ahead, as they lie in memory (`wide`: 16-bit scales two to a word, zero points four);
-    // a lane loads those of GL groups of rows g and g + 8
-    uint32_t sn[2][GL], zn[2][GL];
+    // ---- the scales and zero points of a unit: lane l loads GL of row l / 2 one unit ahead, as they lie in memory (16 bits: two to a word
+    // where they are aligned), and puts them into the warp's shared memory as floats and as pairs to subtract
+    constexpr int GU = NB * NG, GL = GU / 2 > 0 ? GU / 2 : 1, SP = GU + 4;  // groups a unit, a lane; words a row
+    float *const scales = reinterpret_cast<float *>(smem + Q4Shape<X>::FIXED - WARPS * Q4Shape<X>::SCALES) + warp * (Q4Shape<X>::SCALES / 4);
+    uint32_t *const zeros = reinterpret_cast<uint32_t *>(scales) + 16 * SP;
+    uint32_t sn[GL], zn[GL];
 #pragma unroll
-    for (int r = 0; r < 2; r++)
-#pragma unroll
-        for (int i = 0; i < GL; i++) sn[r][i] = zn[r][i] = 0;
+    for (int i = 0; i < GL; i++) sn[i] = zn[i] = 0;
+    const int sj = GU > 1 ? (lane & 1) * GL : 0;
     auto fetch_scales = [&](int chunk, int tile) {
-        const int j = t % (NB * NG / GL) * GL, group = (chunk * wk + kw) * cut.mine * NG + j;
-        if (chunk >= cut.chunks || tile >= tile1 || j >= cut.mine * NG) return;
+        const int group = (chunk * wk + kw) * cut.mine * NG + sj;
+        const long row = tile * 16 + (lane >> 1);
+        if (chunk >= cut.chunks || tile >= tile1 || row >= p.M || group >= groups) return;
+        const long at = row * p.s_ld + group;
+        if (cut.wide) {
+            const uint16_t *s = (const uint16_t *)p.wscale + at;
+            if constexpr (GL == 8) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(s));
+                sn[0] = v.x; sn[1 % GL] = v.y; sn[2 % GL] = v.z; sn[3 % GL] = v.w;
+            } else if constexpr (GL == 4) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(s));
+                sn[0] = v.x; sn[1 % GL] = v.y;
+            } else if constexpr (GL == 2)
+                sn[0] = __ldg(reinterpret_cast<const uint32_t *>(s));
+            else
+                sn[0] = __ldg(s);
+        } else {
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const long row = tile * 16 + r * 8 + g;
-            if (row >= p.M) continue;
-            const long at = row * p.s_ld + group;
-            if (cut.wide && GL > 1) {
-                if (group < groups) {
-                    if (GL == 2) sn[r][0] = __ldg(reinterpret_cast<const uint32_t *>((const unsigned short *)p.wscale + at));
-                    else {
-                        const uint2 v = __ldg(reinterpret_cast<const uint2 *>((const unsigned short *)p.wscale + at));
-                        sn[r][0] = v.x;
-                        sn[r][GL > 1] = v.y;
-                    }
-                }
-            } else {
+            for (int i = 0; i < GL; i++)
+                if (group + i < groups) sn[i] = p.s_dtype == THB_F32 ? __ldg((const uint32_t *)p.wscale + at + i) : __ldg((const uint16_t *)p.wscale + at + i);
+        }
+        if (ZEROS) {
+            const uint8_t *z = p.wzero + row * p.z_ld + group;
+            if (cut.wide && GL == 8) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(z));
+                zn[0] = v.x; zn[1 % GL] = v.y;
+            } else if (cut.wide && GL == 4)
+                zn[0] = __ldg(reinterpret_cast<const uint32_t *>(z));
+            else if (cut.wide && GL == 2)
+                zn[0] = __ldg(reinterpret_cast<const uint16_t *>(z));
+            else {
 #pragma unroll
                 for (int i = 0; i < GL; i++)
-                    if (group + i < groups) sn[r][i] = p.s_dtype == THB_F32 ? __ldg((const uint32_t *)p.wscale + at + i) : __ldg((const unsigned short *)p.wscale + at + i);
-            }
-            if (ZEROS) {
-                const uint8_t *z = p.wzero + row * p.z_ld + group;
-                if (cut.wide && GL == 4) {
-                    if (group < groups) zn[r][0] = __ldg(reinterpret_cast<const uint32_t *>(z));
-                } else if (cut.wide && GL == 2) {
-                    if (group < groups) zn[r][0] = __ldg(reinterpret_cast<const unsigned short *>(z));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < GL; i++)
-                        if (group + i < groups) zn[r][i] = __ldg(z + i);
-                }
+                    if (group + i < groups) zn[i] = __ldg(z + i);
             }
         }
+    };
+    auto put_scales = [&](int chunk) {
+        const int group = (chunk * wk + kw) * cut.mine * NG + sj;
+        float f[GL];
+        if (p.s_dtype == THB_F32) {
+#pragma unroll
+            for (int i = 0; i < GL; i++) f[i] = __uint_as_float(sn[i]);
+        } else {
+            uint32_t h[GL];
+#pragma unroll
+            for (int i = 0; i < GL; i++) h[i] = cut.wide ? sn[i / 2] >> (16 * (i & 1)) : sn[i];
+            if (p.s_dtype == THB_F16) {
+#pragma unroll
+                for (int i = 0; i < GL; i++) f[i] = __half2float(__ushort_as_half((unsigned short)h[i]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < GL; i++) f[i] = __uint_as_float(h[i] << 16);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < GL; i++)  // (what lies behind a row's groups is not a scale; rows behind the last have any, and are not written)
+            scales[(lane >> 1) * SP + sj + i] = group + i < groups ? f[i] : 0.f;
+        if (ZEROS)
+#pragma unroll
+            for (int i = 0; i < GL; i++) zeros[(lane >> 1) * SP + sj + i] = zero_pair<X::BF>(cut.wide ? zn[i / 4] >> (8 * (i & 3)) : zn[i]);
     };
 
     // ---- x of a chunk: as loaded, and as operands
@@ -340,24 +364,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
     for (int chunk = 0; chunk < cut.chunks; chunk++) {
         take_x(chunk);
         for (int step = 0; step < steps; step++) {
-            float sv[2][GL];
-            uint32_t zv[2][GL];
-#pragma unroll
-            for (int r = 0; r < 2; r++)
-#pragma unroll
-                for (int i = 0; i < GL; i++) {
-                    const bool packed = cut.wide && GL > 1;
-                    const uint32_t bits = packed ? sn[r][i / 2] >> (16 * (i & 1)) : sn[r][i];
-                    sv[r][i] = scale_of(bits, p.s_dtype);
-                    if (ZEROS) zv[r][i] = zero_pair<X::BF>(packed ? zn[r][0] >> (8 * i) : zn[r][i]);
-                }
-            // what lies behind a row's groups is not a scale (rows behind the last have any, and are not written)
-            if (((chunk * wk + kw) + 1) * cut.mine * NG > groups) {
-                const int group = (chunk * wk + kw) * cut.mine * NG + t % (NB * NG / GL) * GL;
-#pragma unroll
-                for (int i = 0; i < GL; i++)
-                    if (group + i >= groups) sv[0][i] = sv[1][i] = 0.f;
-            }
+            __syncwarp();  // (all lanes have read the last unit's)
+            put_scales(chunk);
             cp_async_wait<STAGES - 2>();
             __syncwarp();
             fetch();
@@ -368,14 +376,32 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
             const uint32_t at = mine_at + slot * (NB * 1024);
             slot = slot + 1 == STAGES ? 0 : slot + 1;
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            auto block = [&](int n) {
+                // the block's scales and zero points of rows g and g + 8
+                float sc[2][NG];
+                uint32_t zs[2][NG];
 #pragma unroll
-            for (int n = 0; n < NB; n++) {
-                if (n >= cut.mine) break;
+                for (int r = 0; r < 2; r++) {
+                    const int o = (g + 8 * r) * SP + n * NG;
+                    if constexpr (NG == 4) {
+                        const float4 v = *reinterpret_cast<const float4 *>(scales + o);
+                        sc[r][0] = v.x; sc[r][1 % NG] = v.y; sc[r][2 % NG] = v.z; sc[r][3 % NG] = v.w;
+                        if (ZEROS) {
+                            const uint4 z = *reinterpret_cast<const uint4 *>(zeros + o);
+                            zs[r][0] = z.x; zs[r][1 % NG] = z.y; zs[r][2 % NG] = z.z; zs[r][3 % NG] = z.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < NG; j++) {
+                            sc[r][j] = scales[o + j];
+                            if (ZEROS) zs[r][j] = zeros[o + j];
+                        }
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < NG; j++) {
                     float c[4] = {0.f, 0.f, 0.f, 0.f};
                     uint32_t w[2][VW], za[2], zb[2];
-                    float sc[2];
                     constexpr int LINE = NB >= 2 ? 8 : 4;  // pieces of a row in a line
                     const int c0 = n * 4 + j * (GROUP / 32);
 #pragma unroll
@@ -389,9 +415,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
                             w[r][0] = v.x; w[r][1 % VW] = v.y;
                         } else
                             w[r][0] = *reinterpret_cast<const uint32_t *>(src);
-                        const int group = n * NG + j, from = (lane & ~3) | group / GL;
-                        sc[r] = __shfl_sync(0xffffffffu, sv[r][group % GL], from);
-                        za[r] = ZEROS ? __shfl_sync(0xffffffffu, zv[r][group % GL], from) : zero_pair<X::BF>(8);
+                        za[r] = ZEROS ? zs[r][j] : zero_pair<X::BF>(8);
                         zb[r] = X::BF ? 0 : zero_pair_16(za[r]);
                     }
 #pragma unroll
@@ -407,18 +431,31 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
                         }
                     }
 #pragma unroll
-                    for (int q = 0; q < 4; q++) acc[q] = fmaf(c[q], sc[q >> 1], acc[q]);
+                    for (int q = 0; q < 4; q++) acc[q] = fmaf(c[q], sc[q >> 1][j], acc[q]);
                 }
+            };
+            if (cut.mine == NB) {  // (without branches between the blocks, whose instructions then overlap)
+#pragma unroll
+                for (int n = 0; n < NB; n++) block(n);
+            } else {
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+                    if (n < cut.mine) block(n);
             }
             // the tile's parts.  c0, c1: row g, columns 2t and 2t + 1; c2, c3: row g + 8
             float *const parts = part + parity * WARPS * PITCH;
 #pragma unroll
             for (int q = 0; q < 4; q++) parts[warp * PITCH + (2 * t + (q & 1)) * COL + g + (q >> 1) * 8] = acc[q];
-            __syncthreads();  // (the buffers alternate, so that one barrier a step is enough)
+            // Four warps add a tile's parts, two columns each, the other four those of the next tile.  Where a step has one tile, those who
+            // do not add only arrive and go on: everybody waits every other step, and what is waited for includes the end of the other
+            // four's last addition, so that two buffers are enough, and a tile's sums may pass from four warps to the others.
+            const int adding = parity;
+            if (wm > 1) __syncthreads();
+            else if (warp / 4 == adding) asm volatile("bar.sync %0, %1;" ::"r"(1 + parity), "n"(WARPS * 32) : "memory");
+            else asm volatile("bar.arrive %0, %1;" ::"r"(1 + parity), "n"(WARPS * 32) : "memory");
             parity ^= 1;
-            // four warps add a tile's parts, two columns each, and the steps go round the warps
             for (int i = 0; i < wm; i++) {
-                const int turn = (step * wm + i) % (WARPS / 4), local = step * wm + i, tile = tile0 + local;
+                const int turn = wm > 1 ? i & 1 : adding, local = step * wm + i, tile = tile0 + local;
                 const int n = (warp & 3) * 2 + (lane >> 4), row = lane & 15, m = tile * 16 + row;
                 if (warp / 4 != turn || n >= p.N || tile >= tile1) continue;
                 const float *from = parts + i * wk * PITCH + n * COL + row;
@@ -427,7 +464,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
                 float *sum = sums + local * 128 + n * 16 + row;
                 if (chunk > 0) v += *sum;
                 if (chunk + 1 < cut.chunks) {
-                    *sum = v;  // (the same thread comes for it)
+                    *sum = v;
                     continue;
                 }
                 if (m >= (p.M + 7) / 8 * 8 || (p.dtype == THB_F32 && m >= (p.M + 3) / 4 * 4)) continue;
@@ -452,7 +489,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
 template <typename X, int GROUP, bool ZEROS> int launch_q4_group(const Q4Params &p, cudaStream_t st)
 {
     constexpr int NB = Q4Shape<X>::NB, FIXED = Q4Shape<X>::FIXED;
-    constexpr int GL = NB * (128 / GROUP) > 4 ? NB * (128 / GROUP) / 4 : 1;
+    constexpr int GL = NB * (128 / GROUP) / 2 > 0 ? NB * (128 / GROUP) / 2 : 1;
     const auto kern = gemv_q4_kernel<X, GROUP, ZEROS>;
     static int sms[64];
     int dev = 0;
@@ -470,7 +507,8 @@ template <typename X, int GROUP, bool ZEROS> int launch_q4_group(const Q4Params 
     while (c.wk > 1 && c.wk / 2 * NB >= blocks) c.wk /= 2;
     c.chunks = (blocks + c.wk * NB - 1) / (c.wk * NB);
     c.mine = (blocks + c.wk * c.chunks - 1) / (c.wk * c.chunks);
-    c.wide = p.s_dtype != THB_F32 && p.s_ld % GL == 0 && reinterpret_cast<uintptr_t>(p.wscale) % (2 * GL) == 0 && (!p.wzero || (p.z_ld % GL == 0 && reinterpret_cast<uintptr_t>(p.wzero) % GL == 0));
+    c.wide = p.s_dtype != THB_F32 && (c.mine * (128 / GROUP)) % GL == 0 && p.s_ld % GL == 0 && reinterpret_cast<uintptr_t>(p.wscale) % (2 * GL) == 0 &&
+             (!p.wzero || (p.z_ld % GL == 0 && reinterpret_cast<uintptr_t>(p.wzero) % GL == 0));
     int grid = c.tiles < sms[dev] ? c.tiles : sms[dev];
     if (c.chunks > 1 && grid < (c.tiles + Q4_ACC - 1) / Q4_ACC) grid = (c.tiles + Q4_ACC - 1) / Q4_ACC;
     const int most = (c.tiles + grid - 1) / grid;
