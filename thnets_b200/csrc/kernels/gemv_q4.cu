@@ -23,10 +23,10 @@ struct Q4Params {
     int N, K, M, x_ld, y_ld, w_ld, s_ld, z_ld, s_dtype, dtype;
 };
 
-struct XF16 { static constexpr bool BF = false; static constexpr int PARTS = 1; };
-struct XBF16 { static constexpr bool BF = true; static constexpr int PARTS = 1; };
-struct XF32 { static constexpr bool BF = true; static constexpr int PARTS = 3; };
-struct XE4M3 { static constexpr bool BF = false; static constexpr int PARTS = 1; };
+struct XF16 { static constexpr bool BF = false; static constexpr int PARTS = 1, SIZE = 2; };
+struct XBF16 { static constexpr bool BF = true; static constexpr int PARTS = 1, SIZE = 2; };
+struct XF32 { static constexpr bool BF = true; static constexpr int PARTS = 3, SIZE = 4; };
+struct XE4M3 { static constexpr bool BF = false; static constexpr int PARTS = 1, SIZE = 1; };
 
 template <bool BF>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
@@ -81,10 +81,10 @@ __device__ __forceinline__ uint32_t zero_pair_16(uint32_t za)
 template <typename X> struct XVec;
 struct XVec16 {
     uint4 v;
-    __device__ __forceinline__ void load(const void *x, long row, int k, int K)
+    __device__ __forceinline__ void load(const uint8_t *x, int k, int K)
     {
         v = make_uint4(0, 0, 0, 0);
-        if (k < K) v = *reinterpret_cast<const uint4 *>((const uint16_t *)x + row + k);
+        if (k < K) v = *reinterpret_cast<const uint4 *>(x + 2L * k);
     }
     __device__ __forceinline__ void cut(int left)  // values from `left` on (0 < left < 8) lie behind the row
     {
@@ -109,10 +109,10 @@ template <> struct XVec<XE4M3> {
         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
         return (uint32_t)h.x | (uint32_t)h.y << 16;
     }
-    __device__ __forceinline__ void load(const void *x, long row, int k, int K)
+    __device__ __forceinline__ void load(const uint8_t *x, int k, int K)
     {
         v = make_uint2(0, 0);
-        if (k < K) v = *reinterpret_cast<const uint2 *>((const uint8_t *)x + row + k);
+        if (k < K) v = *reinterpret_cast<const uint2 *>(x + k);
     }
     __device__ __forceinline__ void cut(int left)
     {
@@ -130,12 +130,12 @@ template <> struct XVec<XE4M3> {
 };
 template <> struct XVec<XF32> {
     float v[8];
-    __device__ __forceinline__ void load(const void *x, long row, int k, int K)
+    __device__ __forceinline__ void load(const uint8_t *x, int k, int K)
     {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (k + 4 * h < K) f = *reinterpret_cast<const float4 *>((const float *)x + row + k + 4 * h);
+            if (k + 4 * h < K) f = *reinterpret_cast<const float4 *>(x + 4L * (k + 4 * h));
             v[4 * h] = f.x; v[4 * h + 1] = f.y; v[4 * h + 2] = f.z; v[4 * h + 3] = f.w;
         }
     }
@@ -165,322 +165,295 @@ template <> struct XVec<XF32> {
     }
 };
 
-// How a launch is cut, by the shape alone: the warps of a CTA are wk along k times WARPS / wk tiles of 16 rows; a row's blocks of 128 k are
-// walked in `chunks` passes of wk warps by `mine` blocks each.
+// How a launch is cut, by the shape alone: the warps of a CTA are wk along k times WARPS / wk tiles of 32 rows, `mine` blocks of 128 k each.
 struct Q4Cut {
-    int wk, mine, chunks, tiles, wide;  // wide: 16-bit scales, and zero points, are aligned to what a lane loads of them
+    int wk, mine, tiles, wide;  // wide: 16-bit scales, and zero points, are aligned to a block's
 };
-#ifndef Q4W
-#define Q4W 8
-#endif
-static_assert(Q4W == 8, "two groups of four warps");
-constexpr int WARPS = Q4W, Q4_ACC = 64;  // warps a CTA; tiles whose sums a CTA keeps between chunks
-constexpr int COL = 20, PITCH = 8 * COL;  // floats a column, and a warp's part, take in shared memory: no bank twice in the parts' writes
+constexpr int WARPS = 16, NB = 2, STAGES = 2;     // blocks a stage; stages a warp
+constexpr int STAGE = NB * 2048;                  // bytes: 32 rows
+constexpr int COL = 36, PITCH = 8 * COL;          // floats a column, and a warp's part, take in shared memory: no bank twice in the parts' writes
+constexpr int RING = WARPS * STAGES * STAGE, PARTS_AT = RING, SCALES_AT = PARTS_AT + WARPS * PITCH * 4;
+template <int NG> constexpr int SP = NG == 4 ? 12 : NG == 2 ? 10 : 5;  // words a row's scales and zero points take
+template <int NG> constexpr int SMEM = SCALES_AT + WARPS * 32 * SP<NG> * 4;
 
-template <typename X> struct Q4Shape {
-    static constexpr int NB = (X::PARTS == 3 ? 16 : 32) / WARPS;  // blocks a stage at most
-    static constexpr int STAGES = X::PARTS == 3 ? 8 : 4;
-    static constexpr int SCALES = 2 * 16 * (NB * 4 + 4) * 4;      // bytes of scales and zero points a warp
-    static constexpr int RING = WARPS * STAGES * NB * 1024, FIXED = RING + 2 * WARPS * PITCH * 4 + WARPS * SCALES;
-};
-
-// One CTA to an SM owns a range of tiles.  A warp keeps its part of x in registers as B operands and walks the CTA's
-// tiles past it; the codes come through a ring of its own in shared memory, 16 rows by `mine` blocks a stage, by cp.async of 16 bytes (no
-// registers and no barrier between warps: up to 128 KB under way an SM).  The warps' parts are added at a tile's end; where a row has
-// more chunks than one, the sums stay in shared memory until the last, and x of the next chunk is loaded during the last tile of this one.
-// Lane (g = lane / 4, t = lane % 4) holds rows g and g + 8.  Of a block it takes the k of its t: 32 in one vector where a group is 128
-// long, 16 of each of two groups, 8 of each of four, so that a product's k are all of one group.
+// One CTA of sixteen warps to an SM owns a range of tiles.  The codes come through a ring of a warp's own in shared memory, 32 rows by two
+// blocks a stage, by cp.async of 16 bytes (no registers, no barrier between warps: 64 KB under way an SM while as much is multiplied).  x comes
+// from the L1, a block ahead, and each of its operands is multiplied by both 16-row halves of the tile.  Where the tiles are too few for the
+// warps, wk of them share a row's blocks and their parts are added through shared memory; else a warp has whole rows.
+// Lane (g = lane / 4, t = lane % 4) holds rows g, g + 8, g + 16 and g + 24.  Of a block it takes the k of its t: 32 in one vector where a group
+// is 128 long, 16 of each of two groups, 8 of each of four, so that a product's k are all of one group.
 template <typename X, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cut cut)
 {
-    constexpr int NB = Q4Shape<X>::NB, STAGES = Q4Shape<X>::STAGES;
-    constexpr int VW = GROUP / 32, NG = 128 / GROUP;             // words a load, groups a block
-    constexpr int RS = 32 / (NB * 4);                            // rows a warp's cp.async covers (NB = 1: 8, 2: 4, 4: 2)
+    constexpr int VW = GROUP / 32, NG = 128 / GROUP, GU = NB * NG;  // words a load, groups a block, groups a stage
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    float *part = reinterpret_cast<float *>(smem + Q4Shape<X>::RING);  // [2][warps][PITCH]
-    float *sums = reinterpret_cast<float *>(smem + Q4Shape<X>::FIXED);  // [tiles of the CTA][128], where there are chunks
-    const uint32_t ring = smem_u32(smem) + warp * STAGES * NB * 1024;
-
+    const uint32_t ring = smem_u32(smem) + warp * STAGES * STAGE;
     const int tile0 = (int)((long)cut.tiles * blockIdx.x / gridDim.x), tile1 = (int)((long)cut.tiles * (blockIdx.x + 1) / gridDim.x);
     const int wk = cut.wk, wm = WARPS / wk, kw = warp % wk, mw = warp / wk;
-    const int steps = (tile1 - tile0 + wm - 1) / wm;
-    const int groups = (p.K + GROUP - 1) / GROUP, bytes = ((p.K + 1) / 2 + 15) / 16 * 16;
+    const int blocks = (p.K + 127) / 128, groups = (p.K + GROUP - 1) / GROUP, bytes = ((p.K + 1) / 2 + 15) / 16 * 16;
+    const int b0 = kw * cut.mine, b1 = min(blocks, b0 + cut.mine);  // (b0 may be beyond the row: then there is nothing to add)
 
-    // 16-byte pieces of a stage, permuted so that no load of 8, 4 or 2 rows meets a bank twice (rows of 64 bytes lie two to a line)
-    auto piece = [](int row, int c) {
-        const int at = row * (NB * 4) + c, line = at >> 3;
-        const int f = VW == 4 ? (NB >= 2 ? (row & 1) << 2 : 0) : VW == 2 ? (NB >= 2 ? (row & 3) << 1 : (line & 1) << 1) : (NB >= 2 ? row & 7 : line & 3);
-        return (at ^ f) * 16;
-    };
+    // 16-byte pieces of a stage, permuted so that no load of 8, 4 or 2 rows meets a bank twice
+    auto piece = [](int row, int c) { return ((row * 8 + c) ^ (VW == 4 ? (row & 1) << 2 : VW == 2 ? (row & 3) << 1 : row & 7)) * 16; };
 
-    // ---- the codes' loads, STAGES - 1 units (a tile of a chunk) ahead
-    int ftile = tile0 + mw, fchunk = 0, fslot = 0;
-    const int fr = lane / (NB * 4), fc = lane % (NB * 4);
-    const uint8_t *fsrc = p.w;
-    long fstep = 0, fnext = 0;
-    uint32_t fsize = 0;
-    auto seek = [&] {
-        const int o = (fchunk * wk + kw) * cut.mine * 64 + fc * 16;
-        const bool in = fchunk < cut.chunks && fc < cut.mine * 4 && o < bytes;
-        fsize = in ? 16 : 0;
-        fsrc = in ? p.w + (long)(ftile * 16 + fr) * p.w_ld + o : p.w;
-        fstep = in ? (long)RS * p.w_ld : 0;
-        fnext = in ? (long)(wm - 1) * 16 * p.w_ld : 0;
-    };
-    seek();
+    // ---- the codes' loads, a stage ahead of the products; lane: pieces fc of rows fr, fr + 4, ...
+    const int fr = lane >> 3, fc = lane & 7;
+    int ftile = tile0 + mw, fb = b0, fslot = 0;
     auto fetch = [&] {
-        const uint32_t at = ring + fslot * (NB * 1024);
-        if (ftile < tile1 && ftile * 16 + 16 <= p.M) {
+        const uint32_t at = ring + fslot * STAGE;
+        const int o = fb * 64 + fc * 16;
+        const uint8_t *src = p.w + (long)(ftile * 32 + fr) * p.w_ld + o;
+        const bool in = ftile < tile1 && fb + (fc >> 2) < b1 && o < bytes;
+        if (ftile < tile1 && ftile * 32 + 32 <= p.M) {
+            const long step = in ? 4L * p.w_ld : 0;
+            const uint32_t size = in ? 16 : 0;
+            if (!in) src = p.w;
 #pragma unroll
-            for (int i = 0; i < 16 / RS; i++) {
-                cp_async16(at + piece(i * RS + fr, fc), fsrc, fsize);
-                fsrc += fstep;
+            for (int i = 0; i < 8; i++) {
+                cp_async16(at + piece(i * 4 + fr, fc), src, size);
+                src += step;
             }
         } else {  // (rows beyond the last are zeros and not written)
 #pragma unroll
-            for (int i = 0; i < 16 / RS; i++) {
-                const bool in = ftile < tile1 && ftile * 16 + i * RS + fr < p.M;
-                cp_async16(at + piece(i * RS + fr, fc), in ? fsrc : p.w, in ? fsize : 0);
-                fsrc += fstep;
+            for (int i = 0; i < 8; i++) {
+                const bool row = in && ftile * 32 + i * 4 + fr < p.M;
+                cp_async16(at + piece(i * 4 + fr, fc), row ? src + i * 4L * p.w_ld : p.w, row ? 16 : 0);
             }
         }
-        fsrc += fnext;
         cp_async_commit();
-        fslot = fslot + 1 == STAGES ? 0 : fslot + 1;
-        ftile += wm;
-        if (ftile - mw >= tile0 + steps * wm) {
-            ftile = tile0 + mw;
-            fchunk++;
-            seek();
+        fslot ^= 1;
+        fb += NB;
+        if (fb >= b1) {
+            fb = b0;
+            ftile += wm;
         }
     };
-    // ---- the scales and zero points of a unit: lane l loads GL of row l / 2 one unit ahead, as they lie in memory (16 bits: two to a word
-    // where they are aligned), and puts them into the warp's shared memory as floats and as pairs to subtract
-    constexpr int GU = NB * NG, GL = GU / 2 > 0 ? GU / 2 : 1, SP = GU + 4;  // groups a unit, a lane; words a row
-    float *const scales = reinterpret_cast<float *>(smem + Q4Shape<X>::FIXED - WARPS * Q4Shape<X>::SCALES) + warp * (Q4Shape<X>::SCALES / 4);
-    uint32_t *const zeros = reinterpret_cast<uint32_t *>(scales) + 16 * SP;
-    uint32_t sn[GL], zn[GL];
+    // ---- the scales and zero points of a stage: a lane loads those of row `lane`, a stage ahead and as they lie in memory (16 bits: two to a
+    // word where they are aligned), and puts them into the warp's shared memory as floats and as bytes
+    float *const scales = reinterpret_cast<float *>(smem + SCALES_AT) + warp * 32 * SP<NG>;
+    uint32_t sn[GU], zn[GU];
 #pragma unroll
-    for (int i = 0; i < GL; i++) sn[i] = zn[i] = 0;
-    const int sj = GU > 1 ? (lane & 1) * GL : 0;
-    auto fetch_scales = [&](int chunk, int tile) {
-        const int group = (chunk * wk + kw) * cut.mine * NG + sj;
-        const long row = tile * 16 + (lane >> 1);
-        if (chunk >= cut.chunks || tile >= tile1 || row >= p.M || group >= groups) return;
+    for (int i = 0; i < GU; i++) sn[i] = zn[i] = 0;
+    auto fetch_scales = [&](int tile, int b) {
+        const int group = b * NG;
+        const long row = tile * 32 + lane;
+        if (tile >= tile1 || row >= p.M || group >= groups) return;
         const long at = row * p.s_ld + group;
+        const uint8_t *z = ZEROS ? p.wzero + row * p.z_ld + group : nullptr;
         if (cut.wide) {
             const uint16_t *s = (const uint16_t *)p.wscale + at;
-            if constexpr (GL == 8) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(s));
-                sn[0] = v.x; sn[1 % GL] = v.y; sn[2 % GL] = v.z; sn[3 % GL] = v.w;
-            } else if constexpr (GL == 4) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(s));
-                sn[0] = v.x; sn[1 % GL] = v.y;
-            } else if constexpr (GL == 2)
-                sn[0] = __ldg(reinterpret_cast<const uint32_t *>(s));
-            else
-                sn[0] = __ldg(s);
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                if (group + n * NG >= groups) break;
+                if constexpr (NG == 4) {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(s + 4 * n));
+                    sn[2 * n] = v.x; sn[2 * n + 1] = v.y;
+                    if (ZEROS) zn[n] = __ldg(reinterpret_cast<const uint32_t *>(z + 4 * n));
+                } else if constexpr (NG == 2) {
+                    sn[n] = __ldg(reinterpret_cast<const uint32_t *>(s + 2 * n));
+                    if (ZEROS) zn[n] = __ldg(reinterpret_cast<const uint16_t *>(z + 2 * n));
+                } else {
+                    sn[n] = __ldg(s + n);
+                    if (ZEROS) zn[n] = __ldg(z + n);
+                }
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < GL; i++)
-                if (group + i < groups) sn[i] = p.s_dtype == THB_F32 ? __ldg((const uint32_t *)p.wscale + at + i) : __ldg((const uint16_t *)p.wscale + at + i);
-        }
-        if (ZEROS) {
-            const uint8_t *z = p.wzero + row * p.z_ld + group;
-            if (cut.wide && GL == 8) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(z));
-                zn[0] = v.x; zn[1 % GL] = v.y;
-            } else if (cut.wide && GL == 4)
-                zn[0] = __ldg(reinterpret_cast<const uint32_t *>(z));
-            else if (cut.wide && GL == 2)
-                zn[0] = __ldg(reinterpret_cast<const uint16_t *>(z));
-            else {
-#pragma unroll
-                for (int i = 0; i < GL; i++)
-                    if (group + i < groups) zn[i] = __ldg(z + i);
-            }
+            for (int i = 0; i < GU; i++)
+                if (group + i < groups) {
+                    sn[i] = p.s_dtype == THB_F32 ? __ldg((const uint32_t *)p.wscale + at + i) : __ldg((const uint16_t *)p.wscale + at + i);
+                    if (ZEROS) zn[i] = __ldg(z + i);
+                }
         }
     };
-    auto put_scales = [&](int chunk) {
-        const int group = (chunk * wk + kw) * cut.mine * NG + sj;
-        float f[GL];
+    auto put_scales = [&](int b) {
+        float f[GU];
         if (p.s_dtype == THB_F32) {
 #pragma unroll
-            for (int i = 0; i < GL; i++) f[i] = __uint_as_float(sn[i]);
+            for (int i = 0; i < GU; i++) f[i] = __uint_as_float(sn[i]);
         } else {
-            uint32_t h[GL];
+            uint32_t h[GU];
 #pragma unroll
-            for (int i = 0; i < GL; i++) h[i] = cut.wide ? sn[i / 2] >> (16 * (i & 1)) : sn[i];
+            for (int i = 0; i < GU; i++) h[i] = cut.wide && NG > 1 ? sn[i / 2] >> (16 * (i & 1)) : sn[i];
             if (p.s_dtype == THB_F16) {
 #pragma unroll
-                for (int i = 0; i < GL; i++) f[i] = __half2float(__ushort_as_half((unsigned short)h[i]));
+                for (int i = 0; i < GU; i++) f[i] = __half2float(__ushort_as_half((unsigned short)h[i]));
             } else {
 #pragma unroll
-                for (int i = 0; i < GL; i++) f[i] = __uint_as_float(h[i] << 16);
+                for (int i = 0; i < GU; i++) f[i] = __uint_as_float(h[i] << 16);
             }
         }
+        // (what lies behind a row's groups is not a scale; rows behind the last have any, and are not written)
+        if ((b + NB) * NG > groups)
 #pragma unroll
-        for (int i = 0; i < GL; i++)  // (what lies behind a row's groups is not a scale; rows behind the last have any, and are not written)
-            scales[(lane >> 1) * SP + sj + i] = group + i < groups ? f[i] : 0.f;
+            for (int i = 0; i < GU; i++)
+                if (b * NG + i >= groups) f[i] = 0.f;
+        float *to = scales + lane * SP<NG>;
+        if constexpr (GU == 8) {
+            *reinterpret_cast<float4 *>(to) = make_float4(f[0], f[1], f[2], f[3 % GU]);
+            *reinterpret_cast<float4 *>(to + 4) = make_float4(f[4 % GU], f[5 % GU], f[6 % GU], f[7 % GU]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < GU; i++) to[i] = f[i];
+        }
         if (ZEROS)
 #pragma unroll
-            for (int i = 0; i < GL; i++) zeros[(lane >> 1) * SP + sj + i] = zero_pair<X::BF>(cut.wide ? zn[i / 4] >> (8 * (i & 3)) : zn[i]);
+            for (int n = 0; n < NB; n++) {
+                uint32_t z = 0;
+                if (cut.wide) z = zn[n];
+                else
+#pragma unroll
+                    for (int j = 0; j < NG; j++) z |= zn[n * NG + j] << (8 * j);
+                reinterpret_cast<uint32_t *>(to)[GU + n] = z;
+            }
     };
 
-    // ---- x of a chunk: as loaded, and as operands
-    const long xrow = (long)(g < p.N ? g : 0) * p.x_ld;
+    // ---- x: the four vectors of a lane, each loaded again for the next block as soon as it has been taken
+    const uint8_t *const xrow = (const uint8_t *)p.x + (long)(g < p.N ? g : 0) * p.x_ld * X::SIZE;
     const int xk = g < p.N ? p.K : 0;  // (columns beyond the rows of x are zeros)
-    XVec<X> raw[NB][4];
-    uint32_t xb[NB][4][X::PARTS][4];
-    auto x_at = [&](int chunk, int n, int i) { return ((chunk * wk + kw) * cut.mine + n) * 128 + (i / VW) * GROUP + t * 8 * VW + (i % VW) * 8; };
-    auto load_x = [&](int chunk) {
-#pragma unroll
-        for (int n = 0; n < NB; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) raw[n][i].load(p.x, xrow, x_at(chunk, n, i), n < cut.mine ? xk : 0);
-    };
-    auto take_x = [&](int chunk) {
-#pragma unroll
-        for (int n = 0; n < NB; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int left = p.K - x_at(chunk, n, i);
-                if (left > 0 && left < 8) raw[n][i].cut(left);
-                raw[n][i].get(xb[n][i]);
-            }
-    };
+    XVec<X> xv[4];
+    auto x_at = [&](int b, int i) { return b * 128 + (i / VW) * GROUP + t * 8 * VW + (i % VW) * 8; };
 
-    // The weights do not depend on the launch before this one: the first stages are under way while that one drains.
-#pragma unroll 1
-    for (int u = 0; u < STAGES - 1; u++) fetch();
-    fetch_scales(0, tile0 + mw);
+    // The weights do not depend on the launch before this one: the first stage is under way while that one drains.
+    fetch();
+    fetch_scales(tile0 + mw, b0);
     pdl_enter();
-    load_x(0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) xv[i].load(xrow, x_at(b0, i), xk);
 
-    // where this lane's codes of row g lie in a stage: pieces differ in bits 4 to 6 by what their number differs in, then by whole lines
-    const uint32_t mine_at = warp * STAGES * NB * 1024 + piece(g, t * VW / 4) + t * VW % 4 * 4;
-    int slot = 0, parity = 0;
-    for (int chunk = 0; chunk < cut.chunks; chunk++) {
-        take_x(chunk);
-        for (int step = 0; step < steps; step++) {
-            __syncwarp();  // (all lanes have read the last unit's)
-            put_scales(chunk);
-            cp_async_wait<STAGES - 2>();
-            __syncwarp();
-            fetch();
-            const bool last = step == steps - 1;
-            fetch_scales(last ? chunk + 1 : chunk, tile0 + mw + (last ? 0 : (step + 1) * wm));
-            if (last && chunk + 1 < cut.chunks) load_x(chunk + 1);
-
-            const uint32_t at = mine_at + slot * (NB * 1024);
-            slot = slot + 1 == STAGES ? 0 : slot + 1;
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            auto block = [&](int n) {
-                // the block's scales and zero points of rows g and g + 8
-                float sc[2][NG];
-                uint32_t zs[2][NG];
+    // where this lane's codes of row g lie in a stage: pieces differ in bits 4 to 6 by what their number differs in
+    const uint32_t lane_at = warp * STAGES * STAGE + piece(g, t * VW / 4) + t * VW % 4 * 4;
+    int slot = 0;
+    for (int step = tile0; step < tile1; step += wm) {
+        const int tile = step + mw;
+        float acc[2][4];
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const int o = (g + 8 * r) * SP + n * NG;
-                    if constexpr (NG == 4) {
-                        const float4 v = *reinterpret_cast<const float4 *>(scales + o);
-                        sc[r][0] = v.x; sc[r][1 % NG] = v.y; sc[r][2 % NG] = v.z; sc[r][3 % NG] = v.w;
-                        if (ZEROS) {
-                            const uint4 z = *reinterpret_cast<const uint4 *>(zeros + o);
-                            zs[r][0] = z.x; zs[r][1 % NG] = z.y; zs[r][2 % NG] = z.z; zs[r][3 % NG] = z.w;
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) acc[i][q] = 0.f;
+        if (tile < tile1 && b0 < b1)
+            for (int b = b0; b < b1; b += NB) {
+                __syncwarp();  // (all lanes have read the last stage and its scales)
+                put_scales(b);
+                fetch();
+                const bool wraps = b + NB >= b1;
+                fetch_scales(wraps ? tile + wm : tile, wraps ? b0 : b + NB);
+                cp_async_wait<STAGES - 1>();
+                __syncwarp();
+                const uint32_t at = lane_at + slot * STAGE;
+                slot ^= 1;
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    if (b + n >= b1) break;
+                    const int next = b + n + 1 < b1 ? b + n + 1 : b0;
+                    if ((b + n) * 128 + 128 > p.K)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int left = p.K - x_at(b + n, i);
+                            if (left > 0 && left < 8) xv[i].cut(left);
                         }
-                    } else {
+                    // the block's scales and zero points of the lane's four rows
+                    float sc[4][NG];
+                    uint32_t zs[4];
 #pragma unroll
-                        for (int j = 0; j < NG; j++) {
-                            sc[r][j] = scales[o + j];
-                            if (ZEROS) zs[r][j] = zeros[o + j];
-                        }
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < NG; j++) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    uint32_t w[2][VW], za[2], zb[2];
-                    constexpr int LINE = NB >= 2 ? 8 : 4;  // pieces of a row in a line
-                    const int c0 = n * 4 + j * (GROUP / 32);
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        const uint8_t *src = smem + (at ^ c0 % LINE * 16) + c0 / LINE * 128 + r * (8 * NB * 64);
-                        if constexpr (VW == 4) {
-                            const uint4 v = *reinterpret_cast<const uint4 *>(src);
-                            w[r][0] = v.x; w[r][1 % VW] = v.y; w[r][2 % VW] = v.z; w[r][3 % VW] = v.w;
-                        } else if constexpr (VW == 2) {
-                            const uint2 v = *reinterpret_cast<const uint2 *>(src);
-                            w[r][0] = v.x; w[r][1 % VW] = v.y;
+                    for (int r = 0; r < 4; r++) {
+                        const float *from = scales + (g + 8 * r) * SP<NG>;
+                        if constexpr (NG == 4) {
+                            const float4 v = *reinterpret_cast<const float4 *>(from + n * NG);
+                            sc[r][0] = v.x; sc[r][1 % NG] = v.y; sc[r][2 % NG] = v.z; sc[r][3 % NG] = v.w;
                         } else
-                            w[r][0] = *reinterpret_cast<const uint32_t *>(src);
-                        za[r] = ZEROS ? zs[r][j] : zero_pair<X::BF>(8);
-                        zb[r] = X::BF ? 0 : zero_pair_16(za[r]);
+#pragma unroll
+                            for (int j = 0; j < NG; j++) sc[r][j] = from[n * NG + j];
+                        if (ZEROS) zs[r] = reinterpret_cast<const uint32_t *>(from)[GU + n];
                     }
 #pragma unroll
-                    for (int h = 0; h < VW; h++) {
-                        uint32_t a[2][4];
+                    for (int j = 0; j < NG; j++) {
+                        float c[2][4];
+                        uint32_t w[4][VW], za[4], zb[4];
+                        const int c0 = n * 4 + j * (GROUP / 32);
 #pragma unroll
-                        for (int r = 0; r < 2; r++) pairs_of<X::BF>(w[r][h], za[r], zb[r], a[r]);
+                        for (int i = 0; i < 2; i++)
 #pragma unroll
-                        for (int q = X::PARTS - 1; q >= 0; q--) {
-                            const uint32_t(&b)[4] = xb[n][j * VW + h][q];
-                            mma16816<X::BF>(c, a[0][0], a[1][0], a[0][1], a[1][1], b[0], b[1]);
-                            mma16816<X::BF>(c, a[0][2], a[1][2], a[0][3], a[1][3], b[2], b[3]);
+                            for (int q = 0; q < 4; q++) c[i][q] = 0.f;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const uint8_t *src = smem + (at ^ c0 * 16) + r * 1024;
+                            if constexpr (VW == 4) {
+                                const uint4 v = *reinterpret_cast<const uint4 *>(src);
+                                w[r][0] = v.x; w[r][1 % VW] = v.y; w[r][2 % VW] = v.z; w[r][3 % VW] = v.w;
+                            } else if constexpr (VW == 2) {
+                                const uint2 v = *reinterpret_cast<const uint2 *>(src);
+                                w[r][0] = v.x; w[r][1 % VW] = v.y;
+                            } else
+                                w[r][0] = *reinterpret_cast<const uint32_t *>(src);
+                            za[r] = zero_pair<X::BF>(ZEROS ? zs[r] >> (8 * j) : 8);
+                            zb[r] = X::BF ? 0 : zero_pair_16(za[r]);
                         }
+#pragma unroll
+                        for (int h = 0; h < VW; h++) {
+                            uint32_t xb[X::PARTS][4];
+                            xv[j * VW + h].get(xb);
+                            xv[j * VW + h].load(xrow, x_at(next, j * VW + h), xk);
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                uint32_t a[2][4];
+#pragma unroll
+                                for (int r = 0; r < 2; r++) pairs_of<X::BF>(w[2 * i + r][h], za[2 * i + r], zb[2 * i + r], a[r]);
+#pragma unroll
+                                for (int q = X::PARTS - 1; q >= 0; q--) {
+                                    mma16816<X::BF>(c[i], a[0][0], a[1][0], a[0][1], a[1][1], xb[q][0], xb[q][1]);
+                                    mma16816<X::BF>(c[i], a[0][2], a[1][2], a[0][3], a[1][3], xb[q][2], xb[q][3]);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+#pragma unroll
+                            for (int q = 0; q < 4; q++) acc[i][q] = fmaf(c[i][q], sc[2 * i + (q >> 1)][j], acc[i][q]);
                     }
-#pragma unroll
-                    for (int q = 0; q < 4; q++) acc[q] = fmaf(c[q], sc[q >> 1][j], acc[q]);
                 }
-            };
-            if (cut.mine == NB) {  // (without branches between the blocks, whose instructions then overlap)
-#pragma unroll
-                for (int n = 0; n < NB; n++) block(n);
-            } else {
-#pragma unroll
-                for (int n = 0; n < NB; n++)
-                    if (n < cut.mine) block(n);
             }
-            // the tile's parts.  c0, c1: row g, columns 2t and 2t + 1; c2, c3: row g + 8
-            float *const parts = part + parity * WARPS * PITCH;
+        // the results.  acc[i]: rows 16i + g (twice) and 16i + g + 8, columns 2t and 2t + 1
+        auto finish = [&](int n, int m, float v) {
+            if (n >= p.N || m >= (p.M + 7) / 8 * 8 || (p.dtype == THB_F32 && m >= (p.M + 3) / 4 * 4)) return;
+            if (m < p.M) {
+                if (p.x_scale) v *= p.x_scale[n];
+                if (p.scale) v *= p.scale[m];
+                if (p.shift) v += p.shift[m];
+                if (p.act.kind != THB_ACT_NONE)
+                    v = thb_apply_act(v, p.act.kind, p.act.threshold, p.act.value, p.act.alpha, p.act.kind == THB_ACT_PRELU ? p.act.slope[m] : 0.f);
+            } else
+                v = 0.f;  // channels of the padded tail of y are kept at exact zero
+            const long to = (long)n * p.y_ld + m;
+            if (p.dtype == THB_F32) ((float *)p.y)[to] = v;
+            else if (p.dtype == THB_F16) ((__half *)p.y)[to] = __float2half_rn(v);
+            else ((__nv_bfloat16 *)p.y)[to] = __float2bfloat16_rn(v);
+        };
+        // A warp's sums go through its part of shared memory, so that the four of a lane's columns become rows side by side.
+        float *const parts = reinterpret_cast<float *>(smem + PARTS_AT);
+        float *mypart = parts + warp * PITCH;
 #pragma unroll
-            for (int q = 0; q < 4; q++) parts[warp * PITCH + (2 * t + (q & 1)) * COL + g + (q >> 1) * 8] = acc[q];
-            // Four warps add a tile's parts, two columns each, the other four those of the next tile.  Where a step has one tile, those who
-            // do not add only arrive and go on: everybody waits every other step, and what is waited for includes the end of the other
-            // four's last addition, so that two buffers are enough, and a tile's sums may pass from four warps to the others.
-            const int adding = parity;
-            if (wm > 1) __syncthreads();
-            else if (warp / 4 == adding) asm volatile("bar.sync %0, %1;" ::"r"(1 + parity), "n"(WARPS * 32) : "memory");
-            else asm volatile("bar.arrive %0, %1;" ::"r"(1 + parity), "n"(WARPS * 32) : "memory");
-            parity ^= 1;
-            for (int i = 0; i < wm; i++) {
-                const int turn = wm > 1 ? i & 1 : adding, local = step * wm + i, tile = tile0 + local;
-                const int n = (warp & 3) * 2 + (lane >> 4), row = lane & 15, m = tile * 16 + row;
-                if (warp / 4 != turn || n >= p.N || tile >= tile1) continue;
-                const float *from = parts + i * wk * PITCH + n * COL + row;
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) mypart[(2 * t + (q & 1)) * COL + i * 16 + g + (q >> 1) * 8] = acc[i][q];
+        if (wk == 1) {
+            __syncwarp();
+            if (tile < tile1)
+                for (int n = 0; n < p.N; n++) finish(n, tile * 32 + lane, mypart[n * COL + lane]);
+            __syncwarp();
+        } else {
+            __syncthreads();
+            // a warp adds a column of a tile
+            for (int i = warp; i < wm * 8; i += WARPS) {
+                const int n = i % 8;
+                if (n >= p.N || step + i / 8 >= tile1) continue;
+                const float *from = parts + i / 8 * wk * PITCH + n * COL + lane;
                 float v = 0.f;
                 for (int q = 0; q < wk; q++) v += from[q * PITCH];
-                float *sum = sums + local * 128 + n * 16 + row;
-                if (chunk > 0) v += *sum;
-                if (chunk + 1 < cut.chunks) {
-                    *sum = v;
-                    continue;
-                }
-                if (m >= (p.M + 7) / 8 * 8 || (p.dtype == THB_F32 && m >= (p.M + 3) / 4 * 4)) continue;
-                if (m < p.M) {
-                    if (p.x_scale) v *= p.x_scale[n];
-                    if (p.scale) v *= p.scale[m];
-                    if (p.shift) v += p.shift[m];
-                    if (p.act.kind != THB_ACT_NONE)
-                        v = thb_apply_act(v, p.act.kind, p.act.threshold, p.act.value, p.act.alpha, p.act.kind == THB_ACT_PRELU ? p.act.slope[m] : 0.f);
-                } else
-                    v = 0.f;  // channels of the padded tail of y are kept at exact zero
-                const long to = (long)n * p.y_ld + m;
-                if (p.dtype == THB_F32) ((float *)p.y)[to] = v;
-                else if (p.dtype == THB_F16) ((__half *)p.y)[to] = __float2half_rn(v);
-                else ((__nv_bfloat16 *)p.y)[to] = __float2bfloat16_rn(v);
+                finish(n, (step + i / 8) * 32 + lane, v);
             }
+            __syncthreads();
         }
     }
     cp_async_wait<0>();
@@ -488,34 +461,38 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
 
 template <typename X, int GROUP, bool ZEROS> int launch_q4_group(const Q4Params &p, cudaStream_t st)
 {
-    constexpr int NB = Q4Shape<X>::NB, FIXED = Q4Shape<X>::FIXED;
-    constexpr int GL = NB * (128 / GROUP) / 2 > 0 ? NB * (128 / GROUP) / 2 : 1;
+    constexpr int NG = 128 / GROUP;
     const auto kern = gemv_q4_kernel<X, GROUP, ZEROS>;
     static int sms[64];
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return thb_refuse(THB_ERR_UNSUPPORTED, "thb_gemv_q4_fwd: device ordinal above 63");
     if (!sms[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FIXED + Q4_ACC * 512);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM<NG>);
         if (e != cudaSuccess) return thb_note_launch(e, "gemv_q4_kernel attributes");
         sms[dev] = thb_sm_count();
     }
     Q4Cut c;
     const int blocks = (p.K + 127) / 128;
-    c.tiles = (p.M + 15) / 16;
-    c.wk = WARPS;
-    while (c.wk > 1 && c.wk / 2 * NB >= blocks) c.wk /= 2;
-    c.chunks = (blocks + c.wk * NB - 1) / (c.wk * NB);
-    c.mine = (blocks + c.wk * c.chunks - 1) / (c.wk * c.chunks);
-    c.wide = p.s_dtype != THB_F32 && (c.mine * (128 / GROUP)) % GL == 0 && p.s_ld % GL == 0 && reinterpret_cast<uintptr_t>(p.wscale) % (2 * GL) == 0 &&
-             (!p.wzero || (p.z_ld % GL == 0 && reinterpret_cast<uintptr_t>(p.wzero) % GL == 0));
-    int grid = c.tiles < sms[dev] ? c.tiles : sms[dev];
-    if (c.chunks > 1 && grid < (c.tiles + Q4_ACC - 1) / Q4_ACC) grid = (c.tiles + Q4_ACC - 1) / Q4_ACC;
-    const int most = (c.tiles + grid - 1) / grid;
+    c.tiles = (p.M + 31) / 32;
+    // As few warps to a row as keep a CTA's warps equally busy: the blocks that a warp takes one after the other, and two more a tile for the
+    // parts' exchange.
+    const int grid = c.tiles < sms[dev] ? c.tiles : sms[dev], most = (c.tiles + grid - 1) / grid;
+    long best = 0;
+    for (int wk = 1; wk <= WARPS && (wk == 1 || wk < 2 * blocks); wk *= 2) {
+        const long steps = (most + WARPS / wk - 1) / (WARPS / wk), cost = steps * ((blocks + wk - 1) / wk + (wk > 1 ? 2 : 0));
+        if (wk == 1 || cost < best) {
+            best = cost;
+            c.wk = wk;
+        }
+    }
+    c.mine = (blocks + c.wk - 1) / c.wk;
+    c.wide = p.s_dtype != THB_F32 && p.s_ld % NG == 0 && reinterpret_cast<uintptr_t>(p.wscale) % (2 * NG) == 0 &&
+             (!p.wzero || (p.z_ld % NG == 0 && reinterpret_cast<uintptr_t>(p.wzero) % NG == 0));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(WARPS * 32);
-    cfg.dynamicSmemBytes = FIXED + (c.chunks > 1 ? most * 512 : 0);
+    cfg.dynamicSmemBytes = SMEM<NG>;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
