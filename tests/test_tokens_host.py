@@ -189,7 +189,7 @@ def test_paged_attn_refusals(lib):
     for bad in (dict(scratch=None), dict(scratch_bytes=need - 1), dict(scratch=AT + 2)):
         assert call(changed(attn_desc, **bad)) == ARG, bad
     huge = cache_desc(heads=70000, token_stride=70000 * 64, page_stride=16 * 70000 * 64)
-    assert call(changed(attn_desc, cache=huge, q_heads=70000, q_ld=70000 * 64, y_ld=70000 * 64)) == UNSUPPORTED
+    assert call(changed(attn_desc, cache=huge, rows=100000, seq=AT, q_heads=70000, q_ld=70000 * 64, y_ld=70000 * 64)) == UNSUPPORTED
 
 
 def test_paged_attn_scratch_covers_every_split(lib):
