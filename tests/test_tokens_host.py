@@ -183,11 +183,11 @@ def test_paged_attn_refusals(lib):
     for bad in (dict(q=None), dict(y=None), dict(q=AT + 8), dict(y=AT + 2)):
         assert call(attn_desc(), **bad) == ARG, bad
     assert call(changed(attn_desc, rows=0)) == OK
-    # a row of 80 positions is split: scratch is needed
-    need = lib.thb_paged_attn_scratch(C.byref(attn_desc()))
+    # a long row is split among more CTAs than can join it by themselves: scratch is needed
+    need = lib.thb_paged_attn_scratch(C.byref(changed(attn_desc, max_len=100000)))
     assert need > 0 and need % 4 == 0
-    for bad in (dict(scratch=None), dict(scratch_bytes=need - 1), dict(scratch=AT + 2)):
-        assert call(changed(attn_desc, **bad)) == ARG, bad
+    for bad in (dict(scratch=None), dict(scratch_bytes=need - 1), dict(scratch=AT + 8)):
+        assert call(changed(attn_desc, max_len=100000, **bad)) == ARG, bad
     huge = cache_desc(heads=70000, token_stride=70000 * 64, page_stride=16 * 70000 * 64)
     assert call(changed(attn_desc, cache=huge, rows=100000, seq=AT, q_heads=70000, q_ld=70000 * 64, y_ld=70000 * 64)) == UNSUPPORTED
 
