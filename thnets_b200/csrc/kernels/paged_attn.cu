@@ -99,14 +99,14 @@ __device__ __forceinline__ void positions(const AttnParams &p, int row, int &fir
 }
 
 // Shared memory: a warp's ring of STAGES tiles, 16 tokens' keys and then their values.  Tiles of 4 and 8 KB leave room for four and two CTAs
-// of four warps on an SM, larger ones for one.  HT: query heads a CTA takes at most.
+// of four warps on an SM, of 16 and 32 KB for two and one of three.  HT: query heads a CTA takes at most.
 template <typename T, int DP, int HT> struct Shape {
     static constexpr int ROW = DP * (int)sizeof(T), HALF = 16 * ROW, TILE = 2 * HALF;
-    static constexpr int WARPS = TILE <= 8192 ? 4 : TILE == 16384 ? 6 : 3, STAGES = TILE <= 8192 ? 3 : 2;
+    static constexpr int WARPS = TILE <= 8192 ? 4 : 3, STAGES = TILE <= 8192 ? 3 : 2;
     static constexpr int PIECES = ROW / 16;                                                    // 16-byte pieces of a row
     static constexpr int QWORDS = sizeof(T) == 4 ? HT * DP : DP * 4;                           // words of Q
     static constexpr int RING = WARPS * STAGES * TILE, SMEM = RING + QWORDS * 4 + WARPS * 64 + 64 + (sizeof(T) == 4 ? WARPS * HT * 64 : 0);
-    static constexpr int CTAS = TILE <= 4096 ? 4 : TILE <= 8192 ? 2 : 1;
+    static constexpr int CTAS = TILE <= 4096 ? 4 : TILE <= 16384 ? 2 : 1;
 };
 
 template <typename T, int DP, int HT>
