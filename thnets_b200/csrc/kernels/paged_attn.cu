@@ -26,7 +26,6 @@ struct AttnParams {
     float scale;
 };
 
-constexpr int CLUSTER_MOST = 512;  // tokens a CTA of a cluster of sixteen takes at most
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // fp16 holds p only down to 2^-24: there it is p * 2^12, which the division by the sum takes back
@@ -48,6 +47,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a)
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
+}
+__device__ __forceinline__ float exp2_of(float x)  // 2^-22 off at most; results below 2^-126 are zero
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ uint4 ldmatrix4(uint32_t at)
 {
@@ -101,11 +106,12 @@ __device__ __forceinline__ void positions(const AttnParams &p, int row, int &fir
 // Shared memory: a warp's ring of STAGES tiles, 16 tokens' keys and then their values.  Tiles of 4 and 8 KB leave room for four and two CTAs
 // of four warps on an SM, of 16 and 32 KB for two and one of three.  HT: query heads a CTA takes at most.
 template <typename T, int DP, int HT> struct Shape {
-    static constexpr int ROW = DP * (int)sizeof(T), HALF = 16 * ROW, TILE = 2 * HALF;
-    static constexpr int WARPS = TILE <= 8192 ? 4 : 3, STAGES = TILE <= 8192 ? 3 : 2;
-    static constexpr int PIECES = ROW / 16;                                                    // 16-byte pieces of a row
-    static constexpr int QWORDS = sizeof(T) == 4 ? HT * DP : DP * 4;                           // words of Q
-    static constexpr int RING = WARPS * STAGES * TILE, SMEM = RING + QWORDS * 4 + WARPS * 64 + 64 + (sizeof(T) == 4 ? WARPS * HT * 64 : 0);
+    static constexpr int ROW = (DP * (int)sizeof(T) + 127) / 128 * 128, HALF = 16 * ROW, TILE = 2 * HALF;
+    static constexpr int WARPS = TILE <= 8192 ? 4 : 3, STAGES = TILE <= 12288 ? 3 : 2;
+    static constexpr int PIECES = DP * (int)sizeof(T) / 16;                                    // 16-byte pieces of a row
+    static constexpr int QWORDS = sizeof(T) == 4 ? HT * DP : 0;                                // words of Q, where they are not in registers
+    // and the warps' maxima and sums, the CTA's, and the warps' p in fp32
+    static constexpr int RING = WARPS * STAGES * TILE, SMEM = RING + QWORDS * 4 + (WARPS + 1) * HT * 8 + (sizeof(T) == 4 ? WARPS * HT * 64 : 0);
     static constexpr int CTAS = TILE <= 4096 ? 4 : TILE <= 16384 ? 2 : 1;
 };
 
@@ -116,8 +122,7 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int WARPS = S::WARPS, STAGES = S::STAGES, VN = Vec16<T>::N, PIECES = S::PIECES, ROW = S::ROW;
     extern __shared__ __align__(128) uint8_t smem[];
-    uint32_t *const qs = reinterpret_cast<uint32_t *>(smem + S::RING);
-    float *const ms = reinterpret_cast<float *>(smem + S::RING + S::QWORDS * 4), *const ls = ms + WARPS * 8, *const joined = ls + WARPS * 8;
+    float *const qs = reinterpret_cast<float *>(smem + S::RING), *const ms = qs + S::QWORDS, *const ls = ms + WARPS * HT, *const joined = ls + WARPS * HT;
     pdl_enter();
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, dim = p.c.dim;
@@ -125,16 +130,18 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
     const int row = blockIdx.z, chunk = blockIdx.y, kv_head = blockIdx.x / p.head_tiles;
     const int head0 = blockIdx.x % p.head_tiles * HT, heads = min(HT, p.share - head0);
     const int q_head0 = kv_head * p.share + head0;
+    // (where no window moves the chunks the first page is asked for together with the length)
+    const int seq = p.seq ? p.seq[row] : row;
+    const int *table = p.c.table + (long)((unsigned)seq < (unsigned)p.c.sequences ? seq : 0) * p.c.table_ld;
+    const bool whole = p.c.page_len % 16 == 0;
+    const long start = (long)chunk * p.chunk + warp * 16 + (whole ? 0 : lane & 15);
+    int fpage = !p.window && start < (long)p.c.table_ld * p.c.page_len ? __ldg(table + (int)start / p.c.page_len) : 0;
     int first, last;
     positions(p, row, first, last);
     if (last < first) return;
     // tiles begin at multiples of 16, so that one lies in one page where pages are multiples of 16 tokens
     const int origin = first & ~15, begin = origin + chunk * p.chunk, end = min(last, begin + p.chunk);
     if (begin >= last && (chunk > 0 || (p.chunks > 1 && !p.cluster))) return;  // (an empty row's zeros: by the first CTA, or by the join)
-
-    const int seq = p.seq ? p.seq[row] : row;
-    const int *table = p.c.table + (long)((unsigned)seq < (unsigned)p.c.sequences ? seq : 0) * p.c.table_ld;
-    const bool whole = p.c.page_len % 16 == 0;
     const uint32_t ring = smem_u32(smem) + warp * STAGES * S::TILE;
     const long head_at = kv_head * p.c.head_stride;
 
@@ -148,29 +155,43 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
         const int token = whole ? tile : tile + (lane & 15);
         return token < end ? __ldg(table + token / p.c.page_len) : 0;
     };
-    int ftile = begin + warp * 16, fslot = 0, fpage = page_of(ftile);
+    constexpr int COPIES = PIECES / 2;  // of 32 pieces
+    auto row_of = [&](int i) { return (i * 32 + lane) / PIECES; };
+    auto piece_of = [&](int i) { return (i * 32 + lane) % PIECES; };
+    int ftile = begin + warp * 16, fslot = 0;
+    if (p.window) fpage = page_of(ftile);
     uint32_t seen[STAGES];  // tokens that count, of the tiles under way
     auto fetch = [&](uint32_t &mask) {
         mask = 0;
         if (ftile < end) {
-            const int token = ftile + (lane & 15);
-            const bool there = (unsigned)fpage < (unsigned)p.c.pages, ok = there && token >= first && token < end;
-            if (!there && token >= first && token < end) *p.c.status = THB_ERR_ARG;
-            mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-            const long mine = ok ? fpage * p.c.page_stride + (token % p.c.page_len) * p.c.token_stride + head_at : 0;
             const uint32_t to = ring + fslot * S::TILE;
-            constexpr int RS = PIECES >= 32 ? 1 : 32 / PIECES;  // rows a warp's instruction covers
+            if (whole && ftile >= first && ftile + 16 <= end && (unsigned)fpage < (unsigned)p.c.pages) {
+                mask = 0xffffu;
+                const long at = fpage * p.c.page_stride + ftile % p.c.page_len * p.c.token_stride + head_at;
 #pragma unroll
-            for (int i = 0; i < 16; i += RS)
+                for (int i = 0; i < COPIES; i++) {
+                    const int r = row_of(i), c = piece_of(i);
+                    const long o = c * VN < dim ? at + r * p.c.token_stride + c * VN : 0;
+                    const uint32_t size = c * VN < dim ? 16 : 0;
+                    cp_async16(to + key_piece(r, c), (const T *)p.c.k + o, size);
+                    cp_async16(to + S::HALF + value_piece(r, c), (const T *)p.c.v + o, size);
+                }
+            } else {
+                const int token = ftile + (lane & 15);
+                const bool there = (unsigned)fpage < (unsigned)p.c.pages, counts = token >= first && token < end, ok = there && counts;
+                if (!there && counts) *p.c.status = THB_ERR_ARG;
+                mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+                const long mine = ok ? fpage * p.c.page_stride + (token % p.c.page_len) * p.c.token_stride + head_at : 0;
 #pragma unroll
-                for (int h = 0; h < (PIECES > 32 ? PIECES / 32 : 1); h++) {
-                    const int r = i + lane / PIECES % RS, c = h * 32 + lane % PIECES;
+                for (int i = 0; i < COPIES; i++) {
+                    const int r = row_of(i), c = piece_of(i);
                     const long at = __shfl_sync(0xffffffffu, mine, r);
                     const bool in = (mask >> r & 1) && c * VN < dim;
                     const long o = in ? at + c * VN : 0;
                     cp_async16(to + key_piece(r, c), (const T *)p.c.k + o, in ? 16 : 0);
                     cp_async16(to + S::HALF + value_piece(r, c), (const T *)p.c.v + o, in ? 16 : 0);
                 }
+            }
             ftile += WARPS * 16;
             fpage = page_of(ftile);
         }
@@ -180,21 +201,26 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
 #pragma unroll
     for (int i = 0; i < STAGES - 1; i++) fetch(seen[i]);
 
-    // Q: in 16 bits as the B operands beside each piece of the keys, head g's values; in fp32 as rows
+    // Q: in 16 bits as the B operands beside each piece of the keys, in registers: head 8n + g's values; in fp32 as rows in shared memory
+    constexpr int NT = (HT + 7) / 8;
+    uint32_t qb[F32 ? 1 : DP / 16][NT][2];
     if constexpr (F32) {
         for (int i = tid; i < HT * DP; i += WARPS * 32) {
             const int h = i / DP, d = i % DP;
-            reinterpret_cast<float *>(qs)[i] = h < heads && d < dim ? ((const float *)p.q)[(long)row * p.q_ld + (long)(q_head0 + h) * dim + d] : 0.f;
+            qs[i] = h < heads && d < dim ? ((const float *)p.q)[(long)row * p.q_ld + (long)(q_head0 + h) * dim + d] : 0.f;
         }
+        __syncthreads();
     } else {
-        for (int j = warp; j < DP / 16; j += WARPS)
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int d = 16 * j + 8 * i + 2 * t;
-                qs[(j * 2 + i) * 32 + lane] = g < heads && d < dim ? *reinterpret_cast<const uint32_t *>((const T *)p.q + (long)row * p.q_ld + (long)(q_head0 + g) * dim + d) : 0u;
-            }
+        for (int j = 0; j < DP / 16; j++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int d = 16 * j + 8 * i + 2 * t, h = 8 * n + g;
+                    qb[j][n][i] = h < heads && d < dim ? *reinterpret_cast<const uint32_t *>((const T *)p.q + (long)row * p.q_ld + (long)(q_head0 + h) * dim + d) : 0u;
+                }
     }
-    __syncthreads();
 
     const float scale = p.scale * LOG2E;
     int slot = 0;
@@ -215,7 +241,7 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
 
     if constexpr (F32) {
         // lane: half of a token's products (pieces of one parity), then VL tokens' share of 4 values a piece
-        constexpr int VP = PIECES > 32 ? 2 : 1, VL = PIECES >= 32 ? 1 : 2;
+        constexpr int VP = PIECES > 32 ? 2 : 1, VL = PIECES > 16 ? 1 : 2;
         float o[HT][VP][4], m[HT], l[HT];
 #pragma unroll
         for (int h = 0; h < HT; h++) {
@@ -226,7 +252,7 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
 #pragma unroll
                 for (int k = 0; k < 4; k++) o[h][i][k] = 0.f;
         }
-        float *const ps = joined + 16 + warp * HT * 16;  // p of this warp's tile, [HT][16]
+        float *const ps = joined + 2 * HT + warp * HT * 16;  // p of this warp's tile, [HT][16]
         for (int tile = begin + warp * 16; tile < end; tile += WARPS * 16) {
             uint32_t mask;
             const uint8_t *const mem = smem + warp * STAGES * S::TILE + next_tile(mask);
@@ -259,9 +285,9 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                 top = fmaxf(top, m[h]);
                 const float ref = top == -INFINITY ? 0.f : top;  // (nothing seen yet: every p is zero)
-                shrink[h] = exp2f(m[h] - ref);
+                shrink[h] = exp2_of(m[h] - ref);
                 m[h] = top;
-                a = exp2f(a - ref);
+                a = exp2_of(a - ref);
                 l[h] = l[h] * shrink[h] + a;
                 if (!(lane & 1)) ps[h * 16 + mytoken] = a;
             }
@@ -274,7 +300,7 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
                     for (int k = 0; k < 4; k++) o[h][i][k] *= shrink[h];
 #pragma unroll
             for (int i = 0; i < 16; i += VL) {
-                const int r = i + (VL > 1 ? lane >> 4 : 0), c = VL > 1 ? lane & 15 : lane;
+                const int r = i + (VL > 1 ? lane >> 4 : 0), c = VL > 1 ? lane & 15 : PIECES < 32 && lane >= PIECES ? 0 : lane;
                 float4 v[VP];
 #pragma unroll
                 for (int q = 0; q < VP; q++) v[q] = *reinterpret_cast<const float4 *>(mem + S::HALF + value_piece(r, c + 32 * q));
@@ -299,13 +325,13 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
-            if (lane == 0) { ms[warp * 8 + h] = m[h]; ls[warp * 8 + h] = l[h]; }
+            if (lane == 0) { ms[warp * HT + h] = m[h]; ls[warp * HT + h] = l[h]; }
 #pragma unroll
             for (int q = 0; q < VP; q++) {
                 if (VL > 1)
 #pragma unroll
                     for (int k = 0; k < 4; k++) o[h][q][k] += __shfl_xor_sync(0xffffffffu, o[h][q][k], 16);
-                if (VL == 1 || lane < 16)
+                if (lane < PIECES)
                     *reinterpret_cast<float4 *>(mine + h * DP + (lane + 32 * q) * 4) = make_float4(o[h][q][0], o[h][q][1], o[h][q][2], o[h][q][3]);
             }
         }
@@ -314,75 +340,91 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
         const uint32_t ring_at = smem_u32(smem) + warp * STAGES * S::TILE;
         // this lane's rows and pieces for ldmatrix: keys [tokens 0-7, 8-15][values 0-7, 8-15] of 16 values, values the other way round
         const uint32_t key_at = key_piece((lane & 7) + (lane >> 3 & 1) * 8, lane >> 4), value_at = value_piece((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
-        float o[TILES][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        float o[NT][TILES][4], m[NT][2], l[NT][2];
 #pragma unroll
-        for (int i = 0; i < TILES; i++)
+        for (int n = 0; n < NT; n++) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; k++) o[i][k] = 0.f;
+            for (int i = 0; i < TILES; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) o[n][i][k] = 0.f;
+        }
         for (int tile = begin + warp * 16; tile < end; tile += WARPS * 16) {
             uint32_t mask;
             const uint32_t at = ring_at + next_tile(mask);
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) s[n][k] = 0.f;
 #pragma unroll
             for (int j = 0; j < DP / 16; j++) {
                 const uint4 a = ldmatrix4(at + (key_at ^ (j & 3) * 32) + (j >> 2) * 128);
-                mma<T>(s, a.x, a.y, a.z, a.w, qs[j * 64 + lane], qs[j * 64 + 32 + lane]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) mma<T>(s[n], a.x, a.y, a.z, a.w, qb[j][n][0], qb[j][n][1]);
             }
-            // the softmax's running maximum and sum of heads 2t and 2t + 1; a lane has tokens g and g + 8 of the sum
+            // the softmax's running maximum and sum of heads 8n + 2t and the next; a lane has tokens g and g + 8 of the sum
             const bool see0 = mask >> g & 1, see1 = mask >> (g + 8) & 1;
-            float pr[4], shrink[2];
+            uint32_t pb[NT][2][2];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const float a = see0 ? s[h] * scale : -INFINITY, b = see1 ? s[2 + h] * scale : -INFINITY;
-                float top = fmaxf(a, b);
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                top = fmaxf(top, m[h]);
-                const float ref = top == -INFINITY ? 0.f : top;  // (nothing seen yet: every p is zero)
-                shrink[h] = exp2f(m[h] - ref);
-                m[h] = top;
-                pr[h] = exp2f(a - ref + SHIFT<T>);
-                pr[2 + h] = exp2f(b - ref + SHIFT<T>);
-                l[h] = l[h] * shrink[h] + (pr[h] + pr[2 + h]);
-            }
-            if (__any_sync(0xffffffffu, shrink[0] != 1.f || shrink[1] != 1.f))
+            for (int n = 0; n < NT; n++) {
+                float pr[4], shrink[2];
 #pragma unroll
-                for (int i = 0; i < TILES; i++) {
-                    o[i][0] *= shrink[0]; o[i][1] *= shrink[1]; o[i][2] *= shrink[0]; o[i][3] *= shrink[1];
+                for (int h = 0; h < 2; h++) {
+                    const float a = see0 ? s[n][h] * scale : -INFINITY, b = see1 ? s[n][2 + h] * scale : -INFINITY;
+                    float top = fmaxf(a, b);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    top = fmaxf(top, m[n][h]);
+                    const float ref = top == -INFINITY ? 0.f : top;  // (nothing seen yet: every p is zero)
+                    shrink[h] = exp2_of(m[n][h] - ref);
+                    m[n][h] = top;
+                    pr[h] = exp2_of(a - ref + SHIFT<T>);
+                    pr[2 + h] = exp2_of(b - ref + SHIFT<T>);
+                    l[n][h] = l[n][h] * shrink[h] + (pr[h] + pr[2 + h]);
                 }
-            // p as the B operand: both parts of (token, heads 2t, 2t + 1), transposed to (head, tokens 2t, 2t + 1)
-            uint32_t pb[2][2];
+                if (__any_sync(0xffffffffu, shrink[0] != 1.f || shrink[1] != 1.f))
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const uint32_t u = pair16<T>(pr[2 * r], pr[2 * r + 1]);
-                const float2 w = wide16<T>(u);
-                pb[0][r] = transpose8x8(u);
-                pb[1][r] = transpose8x8(pair16<T>(pr[2 * r] - w.x, pr[2 * r + 1] - w.y));
+                    for (int i = 0; i < TILES; i++) {
+                        o[n][i][0] *= shrink[0]; o[n][i][1] *= shrink[1]; o[n][i][2] *= shrink[0]; o[n][i][3] *= shrink[1];
+                    }
+                // p as the B operand: both parts of (token, heads 2t, 2t + 1), transposed to (head, tokens 2t, 2t + 1)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const uint32_t u = pair16<T>(pr[2 * r], pr[2 * r + 1]);
+                    const float2 w = wide16<T>(u);
+                    pb[n][0][r] = transpose8x8(u);
+                    pb[n][1][r] = transpose8x8(pair16<T>(pr[2 * r] - w.x, pr[2 * r + 1] - w.y));
+                }
             }
 #pragma unroll
             for (int i = 0; i < TILES; i++) {
                 const uint4 a = ldmatrix4_trans(at + S::HALF + (value_at ^ (i & 3) * 32) + (i >> 2) * 128);
-                mma<T>(o[i], a.x, a.y, a.z, a.w, pb[1][0], pb[1][1]);
-                mma<T>(o[i], a.x, a.y, a.z, a.w, pb[0][0], pb[0][1]);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    mma<T>(o[n][i], a.x, a.y, a.z, a.w, pb[n][1][0], pb[n][1][1]);
+                    mma<T>(o[n][i], a.x, a.y, a.z, a.w, pb[n][0][0], pb[n][0][1]);
+                }
             }
         }
         cp_async_wait<0>();
         __syncwarp();
-        // o[i]: values 16i + g (twice) and 16i + g + 8, heads 2t and 2t + 1
+        // o[n][i]: values 16i + g (twice) and 16i + g + 8, heads 8n + 2t and the next
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
-            if (g == 0) { ms[warp * 8 + 2 * t + h] = m[h]; ls[warp * 8 + 2 * t + h] = l[h]; }
-        }
+        for (int n = 0; n < NT; n++) {
 #pragma unroll
-        for (int i = 0; i < TILES; i++) {
-            mine[2 * t * DP + 16 * i + g] = o[i][0];
-            mine[(2 * t + 1) * DP + 16 * i + g] = o[i][1];
-            mine[2 * t * DP + 16 * i + g + 8] = o[i][2];
-            mine[(2 * t + 1) * DP + 16 * i + g + 8] = o[i][3];
+            for (int h = 0; h < 2; h++) {
+                l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], 4);
+                l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], 8);
+                l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], 16);
+                if (g == 0) { ms[warp * HT + 8 * n + 2 * t + h] = m[n][h]; ls[warp * HT + 8 * n + 2 * t + h] = l[n][h]; }
+            }
+#pragma unroll
+            for (int i = 0; i < TILES; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) mine[(8 * n + 2 * t + (k & 1)) * DP + 16 * i + g + (k >> 1) * 8] = o[n][i][k];
         }
     }
     __syncthreads();
@@ -397,12 +439,12 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
         const int h = i / DP, d = i % DP;
         float top = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) top = fmaxf(top, ms[w * 8 + h]);
+        for (int w = 0; w < WARPS; w++) top = fmaxf(top, ms[w * HT + h]);
         const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int w = 0; w < WARPS; w++) {
-            const float f = exp2f(ms[w * 8 + h] - ref);
-            sum += f * ls[w * 8 + h];
+            const float f = exp2f(ms[w * HT + h] - ref);
+            sum += f * ls[w * HT + h];
             v += f * reinterpret_cast<const float *>(smem + w * STAGES * S::TILE)[i];
         }
         if (p.chunks == 1) result(h, d, v, sum, top);
@@ -410,7 +452,7 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
             reinterpret_cast<float *>(smem)[i] = v;  // (only this thread reads and writes this value of the first warp's part)
             if (d == 0) {
                 joined[h] = top;
-                joined[8 + h] = sum;
+                joined[HT + h] = sum;
             }
         } else {
             if (d < dim) p.part[(slot_at + h) * dim + d] = v;
@@ -429,7 +471,7 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
         const float ref = top == -INFINITY ? 0.f : top;
         for (int c = 0; c < used; c++) {
             const float f = exp2f(*cluster.map_shared_rank(joined + h, c) - ref);
-            sum += f * *cluster.map_shared_rank(joined + 8 + h, c);
+            sum += f * *cluster.map_shared_rank(joined + HT + h, c);
             v += f * *cluster.map_shared_rank(reinterpret_cast<float *>(smem) + i, c);
         }
         result(h, d, v, sum, top);
@@ -529,13 +571,15 @@ template <typename T, int DP> int launch_dim(const AttnParams &p, int ht, cudaSt
         if (ht == 1) return launch_heads<T, DP, 1>(p, st);
         if (ht == 2) return launch_heads<T, DP, 2>(p, st);
         if (ht == 4) return launch_heads<T, DP, 4>(p, st);
+    } else if constexpr (DP <= 128) {
+        if (ht == 16) return launch_heads<T, DP, 16>(p, st);
     }
     return launch_heads<T, DP, 8>(p, st);
 }
 
 template <typename T> int launch_attn(const AttnParams &p, int ht, cudaStream_t st)
 {
-    const int rc = p.c.dim <= 64 ? launch_dim<T, 64>(p, ht, st) : p.c.dim <= 128 ? launch_dim<T, 128>(p, ht, st) : launch_dim<T, 256>(p, ht, st);
+    const int rc = p.c.dim <= 64 ? launch_dim<T, 64>(p, ht, st) : p.c.dim <= 96 ? launch_dim<T, 96>(p, ht, st) : p.c.dim <= 128 ? launch_dim<T, 128>(p, ht, st) : launch_dim<T, 256>(p, ht, st);
     if (rc || p.chunks == 1 || p.cluster) return rc;
     thb_launch(paged_join_kernel<T>, (unsigned)(p.rows * p.q_heads), 128, st, p);
     return THB_LAUNCH_CHECK("paged_join_kernel");
@@ -549,23 +593,29 @@ Cut cut_of(const thb_paged_attn_desc *d)
 {
     Cut c;
     const int share = d->q_heads / d->cache.heads;
-    c.ht = d->cache.dtype != THB_F32 || share > 4 ? 8 : share > 2 ? 4 : share;
+    c.ht = d->cache.dtype == THB_F32 ? (share > 4 ? 8 : share > 2 ? 4 : share) : share > 8 && d->cache.dim <= 128 ? 16 : 8;
     c.head_tiles = (share + c.ht - 1) / c.ht;
-    // two CTAs to each of a B200's 148 SMs where the rows are max_len long; a tile for each of four warps at least, and at most 1024 tokens,
-    // so that a few long rows among short ones are still many CTAs
+    // One wave of CTAs on a B200's 148 SMs (as many to each as Shape says) where the rows are max_len long; a tile for each of four warps at
+    // least.  Of several rows a CTA takes 2048 tokens at most, so that a few long ones among short ones are still many CTAs.
+    const int row_bytes = d->cache.dim * (d->cache.dtype == THB_F32 ? 4 : 2), slots = 148 * (row_bytes <= 128 ? 4 : row_bytes <= 512 ? 2 : 1);
     const double base = (double)d->rows * d->cache.heads * c.head_tiles;
     const long span = d->window && d->window < d->max_len ? d->window + 15L : d->max_len;  // (from a multiple of 16 on)
-    const long want = base >= 296 ? 1 : (long)(296 / base) + 1;
+    const long want = base >= slots ? 1 : (long)(slots / base);
     auto up = [](long v) { return v < 64 ? 64 : (v + 63) / 64 * 64; };
     long chunk = up((span + want - 1) / want);
-    if (chunk > 1024) chunk = 1024;
+    if (d->rows > 1 && chunk > 2048) chunk = 2048;
     long chunks = (span + chunk - 1) / chunk;
+    // A cluster saves the second launch, but its CTAs come and go together: one wave of them, and of clusters of sixteen one to each
+    // of the device's eight parts (two there took turns: 34 us instead of 23 for sixteen of them); and where it leaves a CTA no more than
+    // 256 tokens, or no more than two launches would.
     c.cluster = 0;
-    if (chunks > 1 && span <= 16 * CLUSTER_MOST) {
-        long n = 2;
-        while (n < chunks && n < 16) n *= 2;
+    const int most = base <= 8 ? 16 : 8;
+    long n = 2;
+    while (n < most && base * n * 2 <= slots && n * 64 < span) n *= 2;
+    const long clustered = up((span + n - 1) / n);
+    if (chunks > 1 && base * n <= slots && clustered <= (chunk > 256 ? chunk : 256)) {
         chunks = n;
-        chunk = up((span + n - 1) / n);
+        chunk = clustered;
         c.cluster = 1;
     }
     c.chunk = (int)chunk;
