@@ -411,7 +411,7 @@ int thb_rope_freq_host(int dim, double base, int scaling, double factor, double 
 /* New tokens into the cache: token t's keys, rotated by pos[t], and its values go to position pos[t] of sequence seq[t]; its queries,
  * rotated the same, to q_out (which may be q).  k, v, q: rows of heads * dim values (parts of one row of q, k and v side by
  * side, if the caller likes).  k = v = NULL: only the queries (the cache's dtype and dim are read, no more); q = q_out = NULL: only
- * the cache.  A token with pos < 0 is a place in a padded batch: nothing of it is read or written.  No two tokens of a call may have the
+ * the cache.  A token with pos < 0 is a place in a padded batch: nothing of it is written.  No two tokens of a call may have the
  * same position of the same sequence, nor two sequences of a call the same page where both write. */
 typedef struct thb_kv_append_desc {
     thb_kv_cache cache;

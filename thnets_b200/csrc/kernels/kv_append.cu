@@ -18,27 +18,51 @@ struct AppendParams {
     int tokens, q_heads, k_ld, v_ld, q_ld, q_out_ld;
 };
 
-template <typename T, int U> __device__ __forceinline__ void get(const T *p, float *v)
-{
-    if constexpr (U == 1) v[0] = dt<T>::ld(p);
-    else Vec16<T>::unpack(*reinterpret_cast<const uint4 *>(p), v);
-}
-template <typename T, int U> __device__ __forceinline__ void put(T *p, const float *v)
-{
-    if constexpr (U == 1) dt<T>::st(p, v[0]);
-    else *reinterpret_cast<uint4 *>(p) = Vec16<T>::pack(v);
-}
+template <typename T, int U> struct Unit;  // what a thread moves at a time: 16 bytes, or one value
+template <typename T> struct Unit<T, 1> {
+    T v;
+    __device__ __forceinline__ void unpack(float *f) const { f[0] = dt<T>::ld(&v); }
+    __device__ __forceinline__ void pack(const float *f) { dt<T>::st(&v, f[0]); }
+};
+template <typename T> struct Unit<T, Vec16<T>::N> {
+    uint4 v;
+    __device__ __forceinline__ void unpack(float *f) const { Vec16<T>::unpack(v, f); }
+    __device__ __forceinline__ void pack(const float *f) { v = Vec16<T>::pack(f); }
+};
 
-// A block has a token.  U: values an access, 16 bytes of them, or one where a vector would hold values of both halves of a pair's
-// or of the rotated and the other part of a head.
-template <typename T, int U>
-__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p)
+// A block has a token.  A thread has the same item of every few heads of q, k and v: a pair of units of both halves, a unit of neighbouring
+// pairs, or units that are not turned; what it turns them by stays in registers.  The first heads' values are asked for before the position
+// and the page are known.  U: values a unit, 16 bytes of them, or one where a vector would hold values of both halves or of the rotated and
+// the other part of a head.
+template <typename T, int U, bool INTER>
+__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, int items, int slots)
 {
+    constexpr int HEADS = 4, PAIRS = U == 1 ? 1 : INTER ? U / 2 : U;  // heads under way a thread; pairs an item
     __shared__ float2 turn[128];
     pdl_enter();
     const int token = blockIdx.x, pos = p.pos[token];
-    if (pos < 0) return;  // a place in a padded batch
     const int rot = p.rope.dim, half = rot / 2, dim = p.c.dim;
+    const int item = threadIdx.x % items, first = threadIdx.x / items, turned = INTER ? (U == 1 ? half : rot / U) : half / U;
+    const bool turns = item < turned, working = first < slots;
+    // the item's first values, and those `apart` behind them where it has two units (interleaved single values: the pair's other one)
+    const int at = turns ? (INTER && U == 1 ? 2 * item : item * U) : rot + (item - turned) * U;
+    const int apart = !turns ? 0 : !INTER ? half : U == 1 ? 1 : 0;
+    const int nq = p.q ? p.q_heads : 0, nk = p.k ? p.c.heads : 0, heads = nq + 2 * nk;
+
+    Unit<T, U> a[HEADS], b[HEADS];
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < HEADS; i++) {
+            const int h = h0 + i * slots;
+            if (!working || h >= heads) break;
+            const T *src = h < nq ? (const T *)p.q + (long)token * p.q_ld + h * dim
+                                  : h < nq + nk ? (const T *)p.k + (long)token * p.k_ld + (h - nq) * dim : (const T *)p.v + (long)token * p.v_ld + (h - nq - nk) * dim;
+            a[i] = *reinterpret_cast<const Unit<T, U> *>(src + at);
+            if (apart) b[i] = *reinterpret_cast<const Unit<T, U> *>(src + at + apart);
+        }
+    };
+    load(first);
+    if (pos < 0) return;  // a place in a padded batch
     for (int i = threadIdx.x; i < half; i += blockDim.x) {
         double t = (double)pos * p.rope.freq[i] * 0.15915494309189533577;  // in turns
         t -= rint(t);
@@ -53,76 +77,69 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p)
         int page = -1;
         if ((unsigned)seq < (unsigned)p.c.sequences && slot < p.c.table_ld) page = p.c.table[(long)seq * p.c.table_ld + slot];
         if ((unsigned)page < (unsigned)p.c.pages) {
-            const long at = page * p.c.page_stride + (pos - slot * p.c.page_len) * p.c.token_stride;
-            ck = (T *)p.c.k + at;
-            cv = (T *)p.c.v + at;
+            const long to = page * p.c.page_stride + (pos - slot * p.c.page_len) * p.c.token_stride;
+            ck = (T *)p.c.k + to;
+            cv = (T *)p.c.v + to;
         } else if (threadIdx.x == 0)
             *p.c.status = THB_ERR_ARG;
     }
     __syncthreads();
+    float2 w[PAIRS];
+#pragma unroll
+    for (int j = 0; j < PAIRS; j++) w[j] = turns ? turn[item * PAIRS + j] : make_float2(1.f, 0.f);
 
-    // a head's items: pairs of vectors (halves) or vectors of pairs (neighbours) that are turned, then vectors that are copied
-    const int turned = p.rope.interleaved ? (U == 1 ? half : rot / U) : half / U, items = turned + (dim - rot) / U, copied = dim / U;
-    auto rotate = [&](const T *src, T *dst, int item) {
-        float a[U], b[U];
-        if (item >= turned) {
-            const int o = rot + (item - turned) * U;
-            get<T, U>(src + o, a);
-            put<T, U>(dst + o, a);
-        } else if (!p.rope.interleaved) {
-            const int o = item * U;
-            get<T, U>(src + o, a);
-            get<T, U>(src + o + half, b);
+    for (int h0 = first; working && h0 < heads;) {
 #pragma unroll
-            for (int j = 0; j < U; j++) {
-                const float2 w = turn[o + j];
-                const float x = a[j], y = b[j];
-                a[j] = x * w.x - y * w.y;
-                b[j] = x * w.y + y * w.x;
-            }
-            put<T, U>(dst + o, a);
-            put<T, U>(dst + o + half, b);
-        } else if constexpr (U == 1) {
-            const float2 w = turn[item];
-            const float x = dt<T>::ld(src + 2 * item), y = dt<T>::ld(src + 2 * item + 1);
-            dt<T>::st(dst + 2 * item, x * w.x - y * w.y);
-            dt<T>::st(dst + 2 * item + 1, x * w.y + y * w.x);
-        } else {
-            const int o = item * U;
-            get<T, U>(src + o, a);
+        for (int i = 0; i < HEADS; i++) {
+            const int h = h0 + i * slots;
+            if (h >= heads) break;
+            T *dst = h < nq ? (T *)p.q_out + (long)token * p.q_out_ld + h * dim
+                            : ck == nullptr ? nullptr : h < nq + nk ? ck + (h - nq) * p.c.head_stride : cv + (h - nq - nk) * p.c.head_stride;
+            if (dst == nullptr) break;  // (the queries come first)
+            if (turns && h < nq + nk) {
+                float x[U], y[U];
+                a[i].unpack(x);
+                if (!INTER || U == 1) {
+                    b[i].unpack(y);
 #pragma unroll
-            for (int j = 0; j < U; j += 2) {
-                const float2 w = turn[(o + j) / 2];
-                const float x = a[j], y = a[j + 1];
-                a[j] = x * w.x - y * w.y;
-                a[j + 1] = x * w.y + y * w.x;
+                    for (int j = 0; j < U; j++) {
+                        const float r = x[j] * w[j % PAIRS].x - y[j] * w[j % PAIRS].y;
+                        y[j] = x[j] * w[j % PAIRS].y + y[j] * w[j % PAIRS].x;
+                        x[j] = r;
+                    }
+                    b[i].pack(y);
+                } else {
+#pragma unroll
+                    for (int j = 0; j + 1 < U; j += 2) {
+                        const float r = x[j] * w[j / 2 % PAIRS].x - x[j + 1] * w[j / 2 % PAIRS].y;
+                        x[j + 1] = x[j] * w[j / 2 % PAIRS].y + x[j + 1] * w[j / 2 % PAIRS].x;
+                        x[j] = r;
+                    }
+                }
+                a[i].pack(x);
             }
-            put<T, U>(dst + o, a);
+            *reinterpret_cast<Unit<T, U> *>(dst + at) = a[i];
+            if (apart) *reinterpret_cast<Unit<T, U> *>(dst + at + apart) = b[i];
         }
-    };
-    const int nq = p.q ? p.q_heads * items : 0, nk = ck ? p.c.heads * items : 0, nv = ck ? p.c.heads * copied : 0;
-    for (int i = threadIdx.x; i < nq + nk + nv; i += blockDim.x) {
-        if (i < nq) {
-            const int h = i / items;
-            rotate((const T *)p.q + (long)token * p.q_ld + h * dim, (T *)p.q_out + (long)token * p.q_out_ld + h * dim, i - h * items);
-        } else if (i < nq + nk) {
-            const int h = (i - nq) / items;
-            rotate((const T *)p.k + (long)token * p.k_ld + h * dim, ck + h * p.c.head_stride, i - nq - h * items);
-        } else {
-            const int h = (i - nq - nk) / copied, o = (i - nq - nk - h * copied) * U;
-            float a[U];
-            get<T, U>((const T *)p.v + (long)token * p.v_ld + h * dim + o, a);
-            put<T, U>(cv + h * p.c.head_stride + o, a);
-        }
+        h0 += HEADS * slots;
+        load(h0);
     }
 }
 
 template <typename T> int launch_append(const AppendParams &p, cudaStream_t st)
 {
     constexpr int VN = Vec16<T>::N;
-    const bool vectors = (p.rope.interleaved ? p.rope.dim : p.rope.dim / 2) % VN == 0;
-    if (vectors) thb_launch(kv_append_kernel<T, VN>, (unsigned)p.tokens, 256, st, p);
-    else thb_launch(kv_append_kernel<T, 1>, (unsigned)p.tokens, 256, st, p);
+    const int rot = p.rope.dim, half = rot / 2, dim = p.c.dim, heads = (p.q ? p.q_heads : 0) + (p.k ? 2 * p.c.heads : 0);
+    const bool inter = p.rope.interleaved, vectors = (inter ? rot : half) % VN == 0;
+    const int u = vectors ? VN : 1, items = (inter ? (vectors ? rot / VN : half) : half / u) + (dim - rot) / u;
+    // threads for as many heads at a time as there are, up to 256 (items is 256 at most)
+    int slots = 256 / items;
+    if (slots > heads) slots = heads;
+    const unsigned block = (unsigned)(items * slots + 31) / 32 * 32;
+    if (vectors && inter) thb_launch(kv_append_kernel<T, VN, true>, (unsigned)p.tokens, block, st, p, items, slots);
+    else if (vectors) thb_launch(kv_append_kernel<T, VN, false>, (unsigned)p.tokens, block, st, p, items, slots);
+    else if (inter) thb_launch(kv_append_kernel<T, 1, true>, (unsigned)p.tokens, block, st, p, items, slots);
+    else thb_launch(kv_append_kernel<T, 1, false>, (unsigned)p.tokens, block, st, p, items, slots);
     return THB_LAUNCH_CHECK("kv_append_kernel");
 }
 
