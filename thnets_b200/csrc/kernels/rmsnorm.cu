@@ -2,7 +2,9 @@
 //     t = x + res;  v = t * r * gain, r = 1/sqrt(mean(t^2) + eps);  q = e4m3(v / (max|v| / 448))
 // One pass: a row's t stay in registers between the reduction and the results.  r is common to a row, so max|v| = r * max|t * gain|
 // and the codes are e4m3(t * gain * (448 / max|t * gain|)): the sum of squares and the maximum are reduced together, and r's
-// rounding does not reach the codes.  HBM-bound on many rows, latency-bound on few.
+// rounding does not reach the codes.  HBM-bound on many rows, and near it by the instructions a value takes; latency-bound on few.
+// us a launch in a chain (share of the measured copy rate): 8192 rows of 4096 in fp16 with residual 43.6 (94 %), to e4m3 41.4 (87 %), without
+// residual 26.9 (76 %); 4096 of 8192 42.8 (96 %); 2048 of 16384 60 (68 %); 262144 of 128 30.6 (67 %); 8192 of 4096 in fp32 90 (91 %).
 #include "tokens.cuh"
 #include <cuda_fp8.h>
 
@@ -27,96 +29,160 @@ __device__ __forceinline__ float max_nan(float a, float b)
 }
 
 // WARP: groups of `lanes` threads (a power of two up to a warp) have a row each; otherwise the whole block shares one.
-// A thread owns vectors tid, tid + threads, ... of its row, VPT at most.  Short rows (VPT <= 2) have the next row under way while
-// one is reduced and written, and keep the gain in registers where there is one vector of it; long ones fill the SM by themselves.
-template <typename T, int VPT, bool WARP>
+// A thread owns vectors tid, tid + threads, ... of its row, VPT at most.  Blocks stay for many rows.  Q: codes are wanted, and with them
+// the row's maximum.
+// What a block reads next is under way while a row is reduced and written: short rows' vectors in registers, longer ones' in a ring of
+// STAGES rows in shared memory by cp.async, of which every thread reads only what it asked for itself, so that nobody waits for another.
+// The gain is in registers where a thread has one vector of it, else in shared memory where that has room.
+template <typename T, int VPT, bool WARP> struct NormShape {
+    static constexpr int VN = Vec16<T>::N;
+    static constexpr int STAGES = WARP ? 0 : VPT <= 4 ? 2 : VPT == 8 ? 1 : 0;
+    static constexpr bool KEEP = VPT <= 2, GLOBAL = VPT == 8 && VN == 8;
+    static int smem(int threads, int nvq, bool res)
+    {
+        return STAGES * VPT * threads * 16 * (res ? 2 : 1) + (KEEP || GLOBAL ? 0 : nvq * VN * 4);
+    }
+};
+template <typename T, int VPT, bool WARP, bool Q>
 __global__ void __launch_bounds__(WARP ? 256 : 512) rmsnorm_kernel(NormParams p, int lanes)
 {
-    constexpr int VN = Vec16<T>::N;
-    constexpr bool AHEAD = VPT <= 2, KEEP = VPT == 1;
-    __shared__ float2 part[2][32];
-    pdl_enter();
+    using S = NormShape<T, VPT, WARP>;
+    constexpr int VN = S::VN, STAGES = S::STAGES;
+    constexpr bool KEEP = S::KEEP;
+    __shared__ float2 part[2][16];
+    extern __shared__ uint4 smem[];
     const int threads = WARP ? lanes : blockDim.x, tid = WARP ? threadIdx.x % lanes : threadIdx.x;
     const int per_block = WARP ? blockDim.x / lanes : 1;
-    const long first = (long)blockIdx.x * per_block + (WARP ? threadIdx.x / lanes : 0), step = (long)gridDim.x * per_block;
     const int nv = (p.C + VN - 1) / VN, nvq = (p.C + 15) / 16 * (16 / VN);  // (8-bit rows are padded to 16 values)
+    const int slot_size = VPT * threads * (p.res ? 2 : 1);                  // vectors a stage: x's, then those of res
+    float4 *const gains = reinterpret_cast<float4 *>(smem + STAGES * slot_size);
+    pdl_enter();
 
-    auto gain_of = [&](int v, float *g) {
+    const long base0 = (long)blockIdx.x * per_block, step = (long)gridDim.x * per_block;
+    const int sub = WARP ? threadIdx.x / lanes : 0;
+    auto stage = [&](int slot, long row) {  // this thread's vectors of a row into its places of the ring
+        if (row < p.rows)
 #pragma unroll
-        for (int j = 0; j < VN; j++) g[j] = p.gain && v * VN + j < p.C ? p.gain[v * VN + j] : 1.f;
+            for (int i = 0; i < VPT; i++) {
+                const int v = tid + i * threads;
+                if (v < nv) {
+                    cp_async16(smem_u32(smem + slot * slot_size + v), (const T *)p.x + row * p.x_ld + v * VN, 16);
+                    if (p.res) cp_async16(smem_u32(smem + slot * slot_size + VPT * threads + v), (const T *)p.res + row * p.res_ld + v * VN, 16);
+                }
+            }
+        cp_async_commit();
     };
-    float kept[VN];
-    if (KEEP) gain_of(tid, kept);
-
-    uint4 xb[VPT], rb[VPT];
-    auto load = [&](long row) {
-        if (row >= p.rows) return;
 #pragma unroll
-        for (int i = 0; i < VPT; i++) {
-            const int v = tid + i * threads;
-            if (v < nv) {
-                xb[i] = *reinterpret_cast<const uint4 *>((const T *)p.x + row * p.x_ld + (long)v * VN);
-                if (p.res) rb[i] = *reinterpret_cast<const uint4 *>((const T *)p.res + row * p.res_ld + (long)v * VN);
+    for (int i = 0; i < STAGES; i++) stage(i, base0 + i * step);
+
+    float kept[KEEP ? VPT : 1][VN];
+    if (KEEP) {
+#pragma unroll
+        for (int i = 0; i < (KEEP ? VPT : 1); i++)
+#pragma unroll
+            for (int j = 0; j < VN; j++) {
+                const int c = (tid + i * threads) * VN + j;
+                kept[i][j] = p.gain && c < p.C ? p.gain[c] : 1.f;
+            }
+    } else if (!S::GLOBAL) {
+        for (int c = threadIdx.x; c < nvq * VN; c += blockDim.x) reinterpret_cast<float *>(gains)[c] = p.gain && c < p.C ? p.gain[c] : 1.f;
+        __syncthreads();
+    }
+    auto gain_of = [&](int i, int v, float (&g)[VN]) {
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int j = 0; j < VN; j++) g[j] = kept[KEEP ? i : 0][j];
+        } else if constexpr (S::GLOBAL) {
+#pragma unroll
+            for (int j = 0; j < VN; j++) g[j] = p.gain && v * VN + j < p.C ? __ldg(p.gain + v * VN + j) : 1.f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < VN / 4; j++) {
+                const float4 f = gains[v * (VN / 4) + j];
+                g[4 * j] = f.x; g[4 * j + 1] = f.y; g[4 * j + 2] = f.z; g[4 * j + 3] = f.w;
             }
         }
     };
-    if (AHEAD) load(first);
-    int parity = 0;
-    // (all threads of a warp take the same number of turns: the reductions name whole warps)
-    const long block_first = (long)blockIdx.x * per_block;
-    for (long base = block_first; base < p.rows; base += step) {
-        const long row = base + (first - block_first);
+
+    uint4 xb = make_uint4(0, 0, 0, 0), rb = xb;
+    auto load = [&](long row) {  // (short rows: one vector a thread)
+        if (row < p.rows && tid < nv) {
+            xb = *reinterpret_cast<const uint4 *>((const T *)p.x + row * p.x_ld + tid * VN);
+            if (p.res) rb = *reinterpret_cast<const uint4 *>((const T *)p.res + row * p.res_ld + tid * VN);
+        }
+    };
+    // (all threads of a block take the same number of turns: the reductions name whole warps)
+    const float inv_c = 1.f / (float)p.C;
+    if (WARP) load(base0 + sub);
+    int parity = 0, slot = 0;
+    for (long base = base0; base < p.rows; base += step) {
+        const long row = base + sub;
         const bool live = row < p.rows;
         float t[VPT][VN], square = 0.f, most = 0.f;
-        if (!AHEAD) load(row);
+        if (STAGES > 0) cp_async_wait<STAGES - 1 < 0 ? 0 : STAGES - 1>();
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
             const int v = tid + i * threads;
             if (live && v < nv) {
-                Vec16<T>::unpack(xb[i], t[i]);
+                if (STAGES > 0) xb = smem[slot * slot_size + v];
+                else if (!WARP) xb = *reinterpret_cast<const uint4 *>((const T *)p.x + row * p.x_ld + v * VN);
+                Vec16<T>::unpack(xb, t[i]);
                 if (p.res) {
                     float r[VN];
-                    Vec16<T>::unpack(rb[i], r);
+                    if (STAGES > 0) rb = smem[slot * slot_size + VPT * threads + v];
+                    else if (!WARP) rb = *reinterpret_cast<const uint4 *>((const T *)p.res + row * p.res_ld + v * VN);
+                    Vec16<T>::unpack(rb, r);
 #pragma unroll
                     for (int j = 0; j < VN; j++) t[i][j] += r[j];
                 }
-                float g[VN];
-                if (!KEEP && p.q) gain_of(v, g);
+                if ((v + 1) * VN > p.C)
 #pragma unroll
-                for (int j = 0; j < VN; j++) {
-                    if (v * VN + j >= p.C) t[i][j] = 0.f;
-                    square = fmaf(t[i][j], t[i][j], square);
-                    if (p.q) most = max_nan(most, fabsf(t[i][j] * (KEEP ? kept[j] : g[j])));
+                    for (int j = 0; j < VN; j++)
+                        if (v * VN + j >= p.C) t[i][j] = 0.f;
+#pragma unroll
+                for (int j = 0; j < VN; j++) square = fmaf(t[i][j], t[i][j], square);
+                if (Q) {
+                    float g[VN];
+                    gain_of(i, v, g);
+#pragma unroll
+                    for (int j = 0; j < VN; j++) most = max_nan(most, fabsf(t[i][j] * g[j]));
                 }
-                if (p.sum) *reinterpret_cast<uint4 *>((T *)p.sum + row * p.sum_ld + (long)v * VN) = Vec16<T>::pack(t[i]);
+                if (p.sum) *reinterpret_cast<uint4 *>((T *)p.sum + row * p.sum_ld + v * VN) = Vec16<T>::pack(t[i]);
             } else {
 #pragma unroll
                 for (int j = 0; j < VN; j++) t[i][j] = 0.f;
             }
         }
-        if (AHEAD) load(row + step);
+        if (WARP) load(row + step);
+        if (STAGES > 0) {
+            stage(slot, base + STAGES * step);
+            slot = slot + 1 == STAGES ? 0 : slot + 1;
+        }
         const int width = WARP ? lanes : 32;
-        for (int o = width / 2; o > 0; o >>= 1) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            if (o >= width) continue;
             square += __shfl_xor_sync(0xffffffffu, square, o);
-            most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+            if (Q) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
         }
         if (!WARP) {
             const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
             if (lane == 0) part[parity][warp] = make_float2(square, most);
             __syncthreads();
-            const float2 o = lane < warps ? part[parity][lane] : make_float2(0.f, 0.f);
+            const float2 o = lane < warps ? part[parity][lane & 15] : make_float2(0.f, 0.f);
             square = o.x;
             most = o.y;
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) {
                 square += __shfl_xor_sync(0xffffffffu, square, k);
-                most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, k));
+                if (Q) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, k));
             }
             parity ^= 1;  // (the buffers alternate, so that one barrier a row is enough)
         }
-        const float r = rsqrtf(square / (float)p.C + p.eps);
-        float scale = 0.f, code = 0.f;
-        if (p.q) {
+        const float r = rsqrtf(square * inv_c + p.eps);
+        float code = 0.f;
+        if (Q) {
+            float scale = 0.f;
             const float top = r * most;
             if (!isfinite(square) || !isfinite(top)) scale = __int_as_float(0x7fc00000);
             else if (top >= 0x1p-100f) {
@@ -129,56 +195,86 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) rmsnorm_kernel(NormParams p,
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
             const int v = tid + i * threads;
-            float g[VN];
-            if (!KEEP) gain_of(v, g);
-            if (p.q && v < nvq) {
+            if (v >= (Q ? nvq : nv)) continue;
+            float g[VN], w[VN];
+            gain_of(i, v, g);
+            if (Q) {
                 uint32_t c[VN / 4];
 #pragma unroll
                 for (int j = 0; j < VN; j += 4) {
-                    float w[4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) w[k] = t[i][j + k] * (KEEP ? kept[j + k] : g[j + k]) * code;
+                    for (int k = 0; k < 4; k++) w[k] = t[i][j + k] * g[j + k] * code;
                     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(w[0], w[1]), __NV_SATFINITE, __NV_E4M3);
                     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(w[2], w[3]), __NV_SATFINITE, __NV_E4M3);
                     c[j / 4] = lo | hi << 16;
                 }
-                uint8_t *at = p.q + row * p.q_ld + (long)v * VN;
+                uint8_t *at = p.q + row * p.q_ld + v * VN;
                 if (VN == 4) *reinterpret_cast<uint32_t *>(at) = c[0];
                 else *reinterpret_cast<uint2 *>(at) = make_uint2(c[0], c[VN / 4 - 1]);
             }
             if (p.y && v < nv) {
-                float w[VN];
 #pragma unroll
-                for (int j = 0; j < VN; j++) w[j] = v * VN + j < p.C ? t[i][j] * r * (KEEP ? kept[j] : g[j]) : 0.f;
-                *reinterpret_cast<uint4 *>((T *)p.y + row * p.y_ld + (long)v * VN) = Vec16<T>::pack(w);
+                for (int j = 0; j < VN; j++) w[j] = t[i][j] * r * g[j];
+                if ((v + 1) * VN > p.C)  // (zeros behind the row, whatever r is)
+#pragma unroll
+                    for (int j = 0; j < VN; j++)
+                        if (v * VN + j >= p.C) w[j] = 0.f;
+                *reinterpret_cast<uint4 *>((T *)p.y + row * p.y_ld + v * VN) = Vec16<T>::pack(w);
             }
         }
     }
 }
 
-template <typename T> int launch_rmsnorm(const NormParams &p, cudaStream_t st)
+template <typename T, int VPT, bool Q> int launch_block(const NormParams &p, cudaStream_t st)
+{
+    using S = NormShape<T, VPT, false>;
+    const auto kern = rmsnorm_kernel<T, VPT, false, Q>;
+    const int nvq = (p.C + 15) / 16 * (16 / S::VN), threads = ((nvq + VPT - 1) / VPT + 31) / 32 * 32, smem = S::smem(threads, nvq, p.res != nullptr);
+    static int sms[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return thb_refuse(THB_ERR_UNSUPPORTED, "thb_rmsnorm_fwd: device ordinal above 63");
+    if (!sms[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        if (e != cudaSuccess) return thb_note_launch(e, "rmsnorm_kernel attributes");
+        sms[dev] = thb_sm_count();
+    }
+    // As many blocks as stay on the device at once, each with many rows: with two vectors a thread so many that 64 KB are under way an SM
+    // (8192 rows of 4096 in 16 bits with a residual: 43.6 us with two blocks of 256 threads, 52.8 with four; without one 30.5 and 26.9; to codes 46.4 and 41.1), with one
+    // as many as there is room for (30000 rows of 1000: 48.7 us with 1024 threads an SM, 40.8 with 2048).
+    const int by_smem = 220 * 1024 / (smem + 2048), by_threads = (VPT == 1 ? 2048 : VPT == 2 && (Q || !p.res) ? 1024 : 512) / threads, resident = by_smem < by_threads ? by_smem : by_threads;
+    const long most = (long)(resident < 1 ? 1 : resident) * sms[dev];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.rows < most ? p.rows : most));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = thb_pdl_enabled() ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, 0);
+    return thb_note_launch(e != cudaSuccess ? e : cudaGetLastError(), "rmsnorm_kernel");
+}
+
+template <typename T, bool Q> int launch_rmsnorm(const NormParams &p, cudaStream_t st)
 {
     constexpr int VN = Vec16<T>::N;
-    const int nv = (p.C + 15) / 16 * (16 / VN), sms = thb_sm_count();
+    const int nv = (p.C + 15) / 16 * (16 / VN);
     if (nv <= 32) {
         int lanes = 1;
         while (lanes < nv) lanes *= 2;
-        const long blocks = (p.rows + 256 / lanes - 1) / (256 / lanes);
-        thb_launch(rmsnorm_kernel<T, 1, true>, (unsigned)(blocks < 8 * sms ? blocks : 8 * sms), 256, st, p, lanes);
+        const long blocks = (p.rows + 256 / lanes - 1) / (256 / lanes), most = 8L * thb_sm_count();
+        thb_launch(rmsnorm_kernel<T, 1, true, Q>, (unsigned)(blocks < most ? blocks : most), 256, st, p, lanes);
         return THB_LAUNCH_CHECK("rmsnorm_kernel");
     }
-    const int vpt = nv <= 512 ? 1 : nv <= 1024 ? 2 : nv <= 2048 ? 4 : nv <= 4096 ? 8 : 16;
-    const int threads = ((nv + vpt - 1) / vpt + 31) / 32 * 32, resident = 2048 / threads;
-    const unsigned grid = (unsigned)(p.rows < (long)resident * sms ? p.rows : (long)resident * sms);
-    switch (vpt) {
-    case 1: thb_launch(rmsnorm_kernel<T, 1, false>, grid, threads, st, p, 0); break;
-    case 2: thb_launch(rmsnorm_kernel<T, 2, false>, grid, threads, st, p, 0); break;
-    case 4: thb_launch(rmsnorm_kernel<T, 4, false>, grid, threads, st, p, 0); break;
-    case 8: thb_launch(rmsnorm_kernel<T, 8, false>, grid, threads, st, p, 0); break;
-    default:
-        if constexpr (VN == 4) thb_launch(rmsnorm_kernel<T, 16, false>, grid, threads, st, p, 0);  // (only rows of fp32 are this many vectors)
-    }
-    return THB_LAUNCH_CHECK("rmsnorm_kernel");
+    if (nv <= 256) return launch_block<T, 1, Q>(p, st);
+    if (nv <= 1024) return launch_block<T, 2, Q>(p, st);
+    if (nv <= 2048) return launch_block<T, 4, Q>(p, st);
+    if (nv <= 4096) return launch_block<T, 8, Q>(p, st);
+    if constexpr (VN == 4) return launch_block<T, 16, Q>(p, st);  // (only rows of fp32 are this many vectors)
+    return THB_ERR_UNSUPPORTED;
 }
 
 }  // namespace
@@ -201,8 +297,8 @@ extern "C" int thb_rmsnorm_fwd(const thb_rmsnorm_desc *d, const void *x, const v
             return thb_refuse(THB_ERR_ARG, "thb_rmsnorm_fwd: a tensor is not 16-byte aligned, or its ld is below C or no multiple of the alignment");
     const NormParams p = {x, res, sum, y, (uint8_t *)q, q_scale, d->gain, d->rows, d->C, d->x_ld, d->res_ld, d->sum_ld, d->y_ld, d->q_ld, d->eps};
     switch (d->dtype) {
-    case THB_F32: return launch_rmsnorm<float>(p, (cudaStream_t)s);
-    case THB_F16: return launch_rmsnorm<__half>(p, (cudaStream_t)s);
-    default: return launch_rmsnorm<__nv_bfloat16>(p, (cudaStream_t)s);
+    case THB_F32: return q ? launch_rmsnorm<float, true>(p, (cudaStream_t)s) : launch_rmsnorm<float, false>(p, (cudaStream_t)s);
+    case THB_F16: return q ? launch_rmsnorm<__half, true>(p, (cudaStream_t)s) : launch_rmsnorm<__half, false>(p, (cudaStream_t)s);
+    default: return q ? launch_rmsnorm<__nv_bfloat16, true>(p, (cudaStream_t)s) : launch_rmsnorm<__nv_bfloat16, false>(p, (cudaStream_t)s);
     }
 }

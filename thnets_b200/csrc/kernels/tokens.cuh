@@ -10,12 +10,16 @@ inline int thb_refuse(int code, const char *why)
 }
 inline bool thb_misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
-inline int thb_sm_count()
+inline int thb_sm_count()  // of the current device
 {
-    int dev = 0, sms = 0;
+    static int sms[64];
+    int dev = 0, n = 0;
     cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms > 0 ? sms : 148;
+    if (dev >= 0 && dev < 64 && sms[dev]) return sms[dev];
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (n <= 0) n = 148;
+    if (dev >= 0 && dev < 64) sms[dev] = n;
+    return n;
 }
 
 // 16 bytes of a type as floats, and back with one rounding each
