@@ -4,6 +4,9 @@
 // pos * freq in fp32 is off by 0.06 rad at a million positions, so the angle is reduced to a fraction of a turn in fp64, once a pair and
 // token for all its heads, and cos and sin are taken of that in fp32.  HBM-bound on prompts (each value read and written once),
 // latency-bound on a decoder's single tokens.
+// us a launch in a chain (share of the measured copy rate), 8192 tokens of 32 + 8 + 8 heads: of 128 in bf16, halves 41.0 (75 %); half of each
+// turned in neighbouring pairs, fp16 41.7 (74 %); of 64 26.7 (58 %); 4096 tokens in fp32 37.1 (83 %).  With a block to a token, which
+// waits for the angles together: 56 / 47 / 34 / 36.
 #include "tokens.cuh"
 #include <math.h>
 
@@ -18,129 +21,151 @@ struct AppendParams {
     int tokens, q_heads, k_ld, v_ld, q_ld, q_out_ld;
 };
 
-template <typename T, int U> struct Unit;  // what a thread moves at a time: 16 bytes, or one value
-template <typename T> struct Unit<T, 1> {
-    T v;
-    __device__ __forceinline__ void unpack(float *f) const { f[0] = dt<T>::ld(&v); }
-    __device__ __forceinline__ void pack(const float *f) { dt<T>::st(&v, f[0]); }
-};
-template <typename T> struct Unit<T, Vec16<T>::N> {
-    uint4 v;
-    __device__ __forceinline__ void unpack(float *f) const { Vec16<T>::unpack(v, f); }
-    __device__ __forceinline__ void pack(const float *f) { v = Vec16<T>::pack(f); }
+// what a lane moves at a time: 16 bytes where halves and parts of a head allow, else 8, 4 or one value
+template <typename T, int U> struct alignas(sizeof(T) * U) Unit {
+    T v[U];
+    __device__ __forceinline__ void unpack(float *f) const
+    {
+        if constexpr (sizeof(T) * U == 16) Vec16<T>::unpack(*reinterpret_cast<const uint4 *>(v), f);
+        else
+#pragma unroll
+            for (int i = 0; i < U; i++) f[i] = dt<T>::ld(v + i);
+    }
+    __device__ __forceinline__ void pack(const float *f)
+    {
+        if constexpr (sizeof(T) * U == 16) *reinterpret_cast<uint4 *>(v) = Vec16<T>::pack(f);
+        else
+#pragma unroll
+            for (int i = 0; i < U; i++) dt<T>::st(v + i, f[i]);
+    }
 };
 
-// A block has a token.  A thread has the same item of every few heads of q, k and v: a pair of units of both halves, a unit of neighbouring
-// pairs, or units that are not turned; what it turns them by stays in registers.  The first heads' values are asked for before the position
-// and the page are known.  U: values a unit, 16 bytes of them, or one where a vector would hold values of both halves or of the rotated and
-// the other part of a head.
+// A warp has every parts-th group of `slots` heads of a token, on its own: where there are many tokens one warp has all heads, so that angles
+// are taken once, where there are few several share them.  A lane has the same item of each of its heads: a pair of units of both halves, a
+// unit of neighbouring pairs, or units that are not turned; the angles it turns by stay in its registers.  HEADS of them are under way, the
+// first before the position and the page are known.
 template <typename T, int U, bool INTER>
-__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, int items, int slots)
+__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, int items, int per, int slots, int parts)
 {
-    constexpr int HEADS = 4, PAIRS = U == 1 ? 1 : INTER ? U / 2 : U;  // heads under way a thread; pairs an item
-    __shared__ float2 turn[128];
+    constexpr int HEADS = 4, PAIRS = U == 1 ? 1 : INTER ? U / 2 : U;  // pairs an item
+    __shared__ float2 turns_of[8][128];
     pdl_enter();
-    const int token = blockIdx.x, pos = p.pos[token];
-    const int rot = p.rope.dim, half = rot / 2, dim = p.c.dim;
-    const int item = threadIdx.x % items, first = threadIdx.x / items, turned = INTER ? (U == 1 ? half : rot / U) : half / U;
-    const bool turns = item < turned, working = first < slots;
-    // the item's first values, and those `apart` behind them where it has two units (interleaved single values: the pair's other one)
-    const int at = turns ? (INTER && U == 1 ? 2 * item : item * U) : rot + (item - turned) * U;
-    const int apart = !turns ? 0 : !INTER ? half : U == 1 ? 1 : 0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long mine = (long)blockIdx.x * 8 + warp;
+    const int token = (int)(mine / parts), part = (int)(mine % parts);
+    if (token >= p.tokens) return;
+    const int pos = p.pos[token], seq = p.k && p.seq ? p.seq[token] : token;
+    const int rot = p.rope.dim, half = rot / 2, dim = p.c.dim, turned = INTER ? (U == 1 ? half : rot / U) : half / U;
     const int nq = p.q ? p.q_heads : 0, nk = p.k ? p.c.heads : 0, heads = nq + 2 * nk;
+    const T *const q = (const T *)p.q + (long)token * p.q_ld, *const k = (const T *)p.k + (long)token * p.k_ld, *const v = (const T *)p.v + (long)token * p.v_ld;
+    T *const q_out = (T *)p.q_out + (long)token * p.q_out_ld, *ck = nullptr, *cv = nullptr;
+    float2 *const turn = turns_of[warp];
+    bool known = false;
 
-    Unit<T, U> a[HEADS], b[HEADS];
-    auto load = [&](int h0) {
+    for (int item0 = 0; item0 < items; item0 += per) {
+        const int item = item0 + lane % per, sub = lane / per;
+        const bool turns = item < turned, working = item < items && sub < slots;
+        // the item's first values, and those `apart` behind them where it has two units (interleaved single values: the pair's other one)
+        const int at = turns ? (INTER && U == 1 ? 2 * item : item * U) : rot + (item - turned) * U;
+        const int apart = !turns ? 0 : !INTER ? half : U == 1 ? 1 : 0;
+        float2 w[PAIRS];
+        for (int h0 = part * slots + sub; h0 - sub < heads; h0 += HEADS * slots * parts) {
+            Unit<T, U> a[HEADS], b[HEADS];
 #pragma unroll
-        for (int i = 0; i < HEADS; i++) {
-            const int h = h0 + i * slots;
-            if (!working || h >= heads) break;
-            const T *src = h < nq ? (const T *)p.q + (long)token * p.q_ld + h * dim
-                                  : h < nq + nk ? (const T *)p.k + (long)token * p.k_ld + (h - nq) * dim : (const T *)p.v + (long)token * p.v_ld + (h - nq - nk) * dim;
-            a[i] = *reinterpret_cast<const Unit<T, U> *>(src + at);
-            if (apart) b[i] = *reinterpret_cast<const Unit<T, U> *>(src + at + apart);
-        }
-    };
-    load(first);
-    if (pos < 0) return;  // a place in a padded batch
-    for (int i = threadIdx.x; i < half; i += blockDim.x) {
-        double t = (double)pos * p.rope.freq[i] * 0.15915494309189533577;  // in turns
-        t -= rint(t);
-        float sn, cs;
-        sincospif((float)(2 * t), &sn, &cs);
-        turn[i] = make_float2(cs * p.rope.magnitude, sn * p.rope.magnitude);
-    }
-    // the token's place: anything beyond the table or the pool is not written
-    T *ck = nullptr, *cv = nullptr;
-    if (p.k) {
-        const int seq = p.seq ? p.seq[token] : token, slot = pos / p.c.page_len;
-        int page = -1;
-        if ((unsigned)seq < (unsigned)p.c.sequences && slot < p.c.table_ld) page = p.c.table[(long)seq * p.c.table_ld + slot];
-        if ((unsigned)page < (unsigned)p.c.pages) {
-            const long to = page * p.c.page_stride + (pos - slot * p.c.page_len) * p.c.token_stride;
-            ck = (T *)p.c.k + to;
-            cv = (T *)p.c.v + to;
-        } else if (threadIdx.x == 0)
-            *p.c.status = THB_ERR_ARG;
-    }
-    __syncthreads();
-    float2 w[PAIRS];
-#pragma unroll
-    for (int j = 0; j < PAIRS; j++) w[j] = turns ? turn[item * PAIRS + j] : make_float2(1.f, 0.f);
-
-    for (int h0 = first; working && h0 < heads;) {
-#pragma unroll
-        for (int i = 0; i < HEADS; i++) {
-            const int h = h0 + i * slots;
-            if (h >= heads) break;
-            T *dst = h < nq ? (T *)p.q_out + (long)token * p.q_out_ld + h * dim
-                            : ck == nullptr ? nullptr : h < nq + nk ? ck + (h - nq) * p.c.head_stride : cv + (h - nq - nk) * p.c.head_stride;
-            if (dst == nullptr) break;  // (the queries come first)
-            if (turns && h < nq + nk) {
-                float x[U], y[U];
-                a[i].unpack(x);
-                if (!INTER || U == 1) {
-                    b[i].unpack(y);
-#pragma unroll
-                    for (int j = 0; j < U; j++) {
-                        const float r = x[j] * w[j % PAIRS].x - y[j] * w[j % PAIRS].y;
-                        y[j] = x[j] * w[j % PAIRS].y + y[j] * w[j % PAIRS].x;
-                        x[j] = r;
-                    }
-                    b[i].pack(y);
-                } else {
-#pragma unroll
-                    for (int j = 0; j + 1 < U; j += 2) {
-                        const float r = x[j] * w[j / 2 % PAIRS].x - x[j + 1] * w[j / 2 % PAIRS].y;
-                        x[j + 1] = x[j] * w[j / 2 % PAIRS].y + x[j + 1] * w[j / 2 % PAIRS].x;
-                        x[j] = r;
-                    }
-                }
-                a[i].pack(x);
+            for (int i = 0; i < HEADS; i++) {
+                const int h = h0 + i * slots * parts;
+                if (!working || h >= heads) break;
+                const T *from = (h < nq ? q + h * dim : h < nq + nk ? k + (h - nq) * dim : v + (h - nq - nk) * dim) + at;
+                a[i] = *reinterpret_cast<const Unit<T, U> *>(from);
+                if (apart) b[i] = *reinterpret_cast<const Unit<T, U> *>(from + apart);
             }
-            *reinterpret_cast<Unit<T, U> *>(dst + at) = a[i];
-            if (apart) *reinterpret_cast<Unit<T, U> *>(dst + at + apart) = b[i];
+            if (!known) {
+                if (pos < 0) return;  // a place in a padded batch
+                // the token's place: anything beyond the table or the pool is not written
+                if (p.k) {
+                    const int slot = pos / p.c.page_len;
+                    int page = -1;
+                    if ((unsigned)seq < (unsigned)p.c.sequences && slot < p.c.table_ld) page = p.c.table[(long)seq * p.c.table_ld + slot];
+                    if ((unsigned)page < (unsigned)p.c.pages) {
+                        const long place = page * p.c.page_stride + (pos - slot * p.c.page_len) * p.c.token_stride;
+                        ck = (T *)p.c.k + place;
+                        cv = (T *)p.c.v + place;
+                    } else if (lane == 0)
+                        *p.c.status = THB_ERR_ARG;
+                }
+                for (int i = lane; i < half; i += 32) {
+                    double t = (double)pos * p.rope.freq[i] * 0.15915494309189533577;  // in turns
+                    t -= rint(t);
+                    float sn, cs;
+                    sincospif((float)(2 * t), &sn, &cs);
+                    turn[i] = make_float2(cs * p.rope.magnitude, sn * p.rope.magnitude);
+                }
+                __syncwarp();
+                known = true;
+            }
+            if (h0 == part * slots + sub)
+#pragma unroll
+                for (int j = 0; j < PAIRS; j++) w[j] = turns ? turn[item * PAIRS + j] : make_float2(1.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < HEADS; i++) {
+                const int h = h0 + i * slots * parts;
+                if (!working || h >= heads) break;
+                T *to = h < nq ? q_out + h * dim : ck == nullptr ? nullptr : h < nq + nk ? ck + (h - nq) * p.c.head_stride : cv + (h - nq - nk) * p.c.head_stride;
+                if (to == nullptr) break;  // (the queries come first)
+                if (turns && h < nq + nk) {
+                    float x[U], y[U];
+                    a[i].unpack(x);
+                    if (!INTER || U == 1) {
+                        b[i].unpack(y);
+#pragma unroll
+                        for (int j = 0; j < U; j++) {
+                            const float r = x[j] * w[j % PAIRS].x - y[j] * w[j % PAIRS].y;
+                            y[j] = x[j] * w[j % PAIRS].y + y[j] * w[j % PAIRS].x;
+                            x[j] = r;
+                        }
+                        b[i].pack(y);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j + 1 < U; j += 2) {
+                            const float r = x[j] * w[j / 2 % PAIRS].x - x[j + 1] * w[j / 2 % PAIRS].y;
+                            x[j + 1] = x[j] * w[j / 2 % PAIRS].y + x[j + 1] * w[j / 2 % PAIRS].x;
+                            x[j] = r;
+                        }
+                    }
+                    a[i].pack(x);
+                }
+                *reinterpret_cast<Unit<T, U> *>(to + at) = a[i];
+                if (apart) *reinterpret_cast<Unit<T, U> *>(to + at + apart) = b[i];
+            }
         }
-        h0 += HEADS * slots;
-        load(h0);
     }
+}
+
+template <typename T, int U> int launch_units(const AppendParams &p, cudaStream_t st)
+{
+    const int rot = p.rope.dim, half = rot / 2, dim = p.c.dim, heads = (p.q ? p.q_heads : 0) + (p.k ? 2 * p.c.heads : 0);
+    const bool inter = p.rope.interleaved;
+    // a head's items, taken at most 32 at a time
+    const int items = (inter ? (U == 1 ? half : rot / U) : half / U) + (dim - rot) / U, turns = (items + 31) / 32, per = (items + turns - 1) / turns, slots = 32 / per;
+    // a warp a token where there are enough of them for 16 warps an SM; else as many as that takes, with a few heads each
+    long parts = 1;
+    const int most = (heads + slots - 1) / slots;
+    while (parts * 2 <= most && p.tokens * parts < 16 * 148L) parts *= 2;
+    const unsigned grid = (unsigned)((p.tokens * parts + 7) / 8);
+    if (inter) thb_launch(kv_append_kernel<T, U, true>, grid, 256, st, p, items, per, slots, (int)parts);
+    else thb_launch(kv_append_kernel<T, U, false>, grid, 256, st, p, items, per, slots, (int)parts);
+    return THB_LAUNCH_CHECK("kv_append_kernel");
 }
 
 template <typename T> int launch_append(const AppendParams &p, cudaStream_t st)
 {
     constexpr int VN = Vec16<T>::N;
-    const int rot = p.rope.dim, half = rot / 2, dim = p.c.dim, heads = (p.q ? p.q_heads : 0) + (p.k ? 2 * p.c.heads : 0);
-    const bool inter = p.rope.interleaved, vectors = (inter ? rot : half) % VN == 0;
-    const int u = vectors ? VN : 1, items = (inter ? (vectors ? rot / VN : half) : half / u) + (dim - rot) / u;
-    // threads for as many heads at a time as there are, up to 256 (items is 256 at most)
-    int slots = 256 / items;
-    if (slots > heads) slots = heads;
-    const unsigned block = (unsigned)(items * slots + 31) / 32 * 32;
-    if (vectors && inter) thb_launch(kv_append_kernel<T, VN, true>, (unsigned)p.tokens, block, st, p, items, slots);
-    else if (vectors) thb_launch(kv_append_kernel<T, VN, false>, (unsigned)p.tokens, block, st, p, items, slots);
-    else if (inter) thb_launch(kv_append_kernel<T, 1, true>, (unsigned)p.tokens, block, st, p, items, slots);
-    else thb_launch(kv_append_kernel<T, 1, false>, (unsigned)p.tokens, block, st, p, items, slots);
-    return THB_LAUNCH_CHECK("kv_append_kernel");
+    const int unit = p.rope.interleaved ? p.rope.dim : p.rope.dim / 2;  // what whole units have to make up (0: nothing is turned)
+    if (unit % VN == 0) return launch_units<T, VN>(p, st);
+    if constexpr (VN == 8)
+        if (unit % 4 == 0) return launch_units<T, 4>(p, st);
+    if (unit % 2 == 0) return launch_units<T, 2>(p, st);
+    return launch_units<T, 1>(p, st);
 }
 
 }  // namespace
