@@ -7,6 +7,12 @@
 // A code becomes q - z in 16 bits exactly (an integer of 5 bits): or'ed into the mantissa of 1024 (fp16; bf16: 128), then z + 1024 is
 // subtracted.  Products and their sums are exact or fp32, a group's sum takes its scale in fp32.  x in fp32 is three bf16 parts
 // (8 + 8 + 8 bits), each multiplied; e4m3 codes are fp16 numbers.
+// What bounds it: the instructions a weight takes, 9 (fp16) or 11 (bf16) for 8 weights to unpack them, as many again for everything else; the
+// half-rate integer pipe is the busiest.  us a call in a chain (of the measured copy rate): 4096->128000, one row, bf16 groups of 128 53.9
+// (5.0 TB/s, 77 %); 4096->32003, four rows of e4m3, groups of 32 23.7 (48 %); 14336->4096, one row, fp16 10.2 (46 %); 9216->4096, eight rows,
+// bf16 groups of 64 with zero points 10.3 (31 %); 25088->4096, three rows, fp32 39 (21 %: 300 of its instructions a block take x apart).
+// Before: codes straight from global memory into registers 164 us for the 4096->32003, x in registers and tiles of 16 rows 31, x from
+// the L1 27.
 #include "tokens.cuh"
 #include <cuda_fp8.h>
 
@@ -167,14 +173,14 @@ template <> struct XVec<XF32> {
 
 // How a launch is cut, by the shape alone: the warps of a CTA are wk along k times WARPS / wk tiles of 32 rows, `mine` blocks of 128 k each.
 struct Q4Cut {
-    int wk, mine, tiles, wide;  // wide: 16-bit scales, and zero points, are aligned to a block's
+    int wk, mine, tiles, wide;  // wide: 16-bit scales, and zero points, are aligned to what a block has of them (1), or to SG (2)
 };
 constexpr int WARPS = 16, NB = 2, STAGES = 2;     // blocks a stage; stages a warp
 constexpr int STAGE = NB * 2048;                  // bytes: 32 rows
 constexpr int COL = 36, PITCH = 8 * COL;          // floats a column, and a warp's part, take in shared memory: no bank twice in the parts' writes
 constexpr int RING = WARPS * STAGES * STAGE, PARTS_AT = RING, SCALES_AT = PARTS_AT + WARPS * PITCH * 4;
-template <int NG> constexpr int SP = NG == 4 ? 12 : NG == 2 ? 10 : 5;  // words a row's scales and zero points take
-template <int NG> constexpr int SMEM = SCALES_AT + WARPS * 32 * SP<NG> * 4;
+constexpr int SG = 8, SP = 12;                    // groups a row whose scales a warp has at a time; words that they and their zero points take
+constexpr int X_AT = SCALES_AT + WARPS * 32 * SP * 4, X_MOST = 227 * 1024 - 1024 - X_AT;  // x in operand order, where it fits
 
 // One CTA of sixteen warps to an SM owns a range of tiles.  The codes come through a ring of a warp's own in shared memory, 32 rows by two
 // blocks a stage, by cp.async of 16 bytes (no registers, no barrier between warps: 64 KB under way an SM while as much is multiplied).  x comes
@@ -182,10 +188,10 @@ template <int NG> constexpr int SMEM = SCALES_AT + WARPS * 32 * SP<NG> * 4;
 // warps, wk of them share a row's blocks and their parts are added through shared memory; else a warp has whole rows.
 // Lane (g = lane / 4, t = lane % 4) holds rows g, g + 8, g + 16 and g + 24.  Of a block it takes the k of its t: 32 in one vector where a group
 // is 128 long, 16 of each of two groups, 8 of each of four, so that a product's k are all of one group.
-template <typename X, int GROUP, bool ZEROS>
+template <typename X, int GROUP, bool ZEROS, bool XS>
 __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cut cut)
 {
-    constexpr int VW = GROUP / 32, NG = 128 / GROUP, GU = NB * NG;  // words a load, groups a block, groups a stage
+    constexpr int VW = GROUP / 32, NG = 128 / GROUP, SB = SG / NG;  // words a load, groups a block, blocks whose scales are at hand
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t ring = smem_u32(smem) + warp * STAGES * STAGE;
@@ -200,127 +206,150 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
     // ---- the codes' loads, a stage ahead of the products; lane: pieces fc of rows fr, fr + 4, ...
     const int fr = lane >> 3, fc = lane & 7;
     int ftile = tile0 + mw, fb = b0, fslot = 0;
+    const uint8_t *fsrc = p.w;
+    long frow = 0;
+    const uint32_t fto = ring + piece(fr, fc), fto4 = ring + piece(fr + 4, fc) - 512;  // (rows i * 4 + fr: even and odd i)
+    auto seek = [&] {
+        const bool any = ftile < tile1 && fb + (fc >> 2) < b1;
+        fsrc = any ? p.w + (long)(ftile * 32 + fr) * p.w_ld + fb * 64 + fc * 16 : p.w;
+        frow = any ? 4L * p.w_ld : 0;
+    };
+    seek();
     auto fetch = [&] {
-        const uint32_t at = ring + fslot * STAGE;
         const int o = fb * 64 + fc * 16;
-        const uint8_t *src = p.w + (long)(ftile * 32 + fr) * p.w_ld + o;
-        const bool in = ftile < tile1 && fb + (fc >> 2) < b1 && o < bytes;
-        if (ftile < tile1 && ftile * 32 + 32 <= p.M) {
-            const long step = in ? 4L * p.w_ld : 0;
-            const uint32_t size = in ? 16 : 0;
-            if (!in) src = p.w;
+        const uint32_t size = ftile < tile1 && fb + (fc >> 2) < b1 && o < bytes ? 16 : 0, at = fslot * STAGE;
+        const uint8_t *src = size ? fsrc : p.w;
+        if (ftile * 32 + 32 <= p.M) {
+            const long step = size ? frow : 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                cp_async16(at + piece(i * 4 + fr, fc), src, size);
+                cp_async16((i & 1 ? fto4 : fto) + at + i * 512, src, size);
                 src += step;
             }
         } else {  // (rows beyond the last are zeros and not written)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const bool row = in && ftile * 32 + i * 4 + fr < p.M;
-                cp_async16(at + piece(i * 4 + fr, fc), row ? src + i * 4L * p.w_ld : p.w, row ? 16 : 0);
+                const bool row = size && ftile * 32 + i * 4 + fr < p.M;
+                cp_async16((i & 1 ? fto4 : fto) + at + i * 512, row ? src + i * frow : p.w, row ? 16 : 0);
             }
         }
         cp_async_commit();
         fslot ^= 1;
         fb += NB;
+        fsrc += NB * 64;
         if (fb >= b1) {
             fb = b0;
             ftile += wm;
+            seek();
         }
     };
-    // ---- the scales and zero points of a stage: a lane loads those of row `lane`, a stage ahead and as they lie in memory (16 bits: two to a
-    // word where they are aligned), and puts them into the warp's shared memory as floats and as bytes
-    float *const scales = reinterpret_cast<float *>(smem + SCALES_AT) + warp * 32 * SP<NG>;
-    uint32_t sn[GU], zn[GU];
+    // ---- the scales and zero points of SG groups (SB blocks): a lane loads those of row `lane`, SB blocks ahead and as they lie in memory (16
+    // bits: two to a word where they are aligned), and puts them into the warp's shared memory as floats and as bytes
+    float *const scales = reinterpret_cast<float *>(smem + SCALES_AT) + warp * 32 * SP;
+    uint32_t sn[SG], zn[SG];
 #pragma unroll
-    for (int i = 0; i < GU; i++) sn[i] = zn[i] = 0;
+    for (int i = 0; i < SG; i++) sn[i] = zn[i] = 0;
     auto fetch_scales = [&](int tile, int b) {
-        const int group = b * NG;
+        const int group = b * NG, left = min(groups, b1 * NG) - group;
         const long row = tile * 32 + lane;
-        if (tile >= tile1 || row >= p.M || group >= groups) return;
+        if (tile >= tile1 || row >= p.M || left <= 0) return;
         const long at = row * p.s_ld + group;
         const uint8_t *z = ZEROS ? p.wzero + row * p.z_ld + group : nullptr;
-        if (cut.wide) {
-            const uint16_t *s = (const uint16_t *)p.wscale + at;
+        if (cut.wide == 2 && left >= SG) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)p.wscale + at));
+            sn[0] = v.x; sn[1] = v.y; sn[2] = v.z; sn[3] = v.w;
+            if (ZEROS) {
+                const uint2 u = __ldg(reinterpret_cast<const uint2 *>(z));
+                zn[0] = u.x; zn[1] = u.y;
+            }
+        } else if (cut.wide && NG > 1) {
 #pragma unroll
-            for (int n = 0; n < NB; n++) {
-                if (group + n * NG >= groups) break;
+            for (int n = 0; n < SB; n++) {
+                if (n * NG >= left) break;
+                const uint16_t *s = (const uint16_t *)p.wscale + at + n * NG;
                 if constexpr (NG == 4) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(s + 4 * n));
+                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(s));
                     sn[2 * n] = v.x; sn[2 * n + 1] = v.y;
-                    if (ZEROS) zn[n] = __ldg(reinterpret_cast<const uint32_t *>(z + 4 * n));
-                } else if constexpr (NG == 2) {
-                    sn[n] = __ldg(reinterpret_cast<const uint32_t *>(s + 2 * n));
-                    if (ZEROS) zn[n] = __ldg(reinterpret_cast<const uint16_t *>(z + 2 * n));
+                    if (ZEROS) zn[n] = __ldg(reinterpret_cast<const uint32_t *>(z + n * NG));
                 } else {
-                    sn[n] = __ldg(s + n);
-                    if (ZEROS) zn[n] = __ldg(z + n);
+                    sn[n] = __ldg(reinterpret_cast<const uint32_t *>(s));
+                    if (ZEROS) zn[n] = __ldg(reinterpret_cast<const uint16_t *>(z + n * NG));
                 }
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < GU; i++)
-                if (group + i < groups) {
+            for (int i = 0; i < SG; i++)
+                if (i < left) {
                     sn[i] = p.s_dtype == THB_F32 ? __ldg((const uint32_t *)p.wscale + at + i) : __ldg((const uint16_t *)p.wscale + at + i);
                     if (ZEROS) zn[i] = __ldg(z + i);
                 }
         }
     };
     auto put_scales = [&](int b) {
-        float f[GU];
+        const int left = min(groups, b1 * NG) - b * NG;
+        const bool full = cut.wide == 2 && left >= SG, packed = full || (cut.wide && NG > 1);
+        float f[SG];
         if (p.s_dtype == THB_F32) {
 #pragma unroll
-            for (int i = 0; i < GU; i++) f[i] = __uint_as_float(sn[i]);
+            for (int i = 0; i < SG; i++) f[i] = __uint_as_float(sn[i]);
         } else {
-            uint32_t h[GU];
+            uint32_t h[SG];
 #pragma unroll
-            for (int i = 0; i < GU; i++) h[i] = cut.wide && NG > 1 ? sn[i / 2] >> (16 * (i & 1)) : sn[i];
+            for (int i = 0; i < SG; i++) h[i] = packed ? sn[i / 2] >> (16 * (i & 1)) : sn[i];
             if (p.s_dtype == THB_F16) {
 #pragma unroll
-                for (int i = 0; i < GU; i++) f[i] = __half2float(__ushort_as_half((unsigned short)h[i]));
+                for (int i = 0; i < SG; i++) f[i] = __half2float(__ushort_as_half((unsigned short)h[i]));
             } else {
 #pragma unroll
-                for (int i = 0; i < GU; i++) f[i] = __uint_as_float(h[i] << 16);
+                for (int i = 0; i < SG; i++) f[i] = __uint_as_float(h[i] << 16);
             }
         }
-        // (what lies behind a row's groups is not a scale; rows behind the last have any, and are not written)
-        if ((b + NB) * NG > groups)
+        if (left < SG)  // (what lies behind a row's groups is not a scale; rows behind the last have any, and are not written)
 #pragma unroll
-            for (int i = 0; i < GU; i++)
-                if (b * NG + i >= groups) f[i] = 0.f;
-        float *to = scales + lane * SP<NG>;
-        if constexpr (GU == 8) {
-            *reinterpret_cast<float4 *>(to) = make_float4(f[0], f[1], f[2], f[3 % GU]);
-            *reinterpret_cast<float4 *>(to + 4) = make_float4(f[4 % GU], f[5 % GU], f[6 % GU], f[7 % GU]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < GU; i++) to[i] = f[i];
+            for (int i = 0; i < SG; i++)
+                if (i >= left) f[i] = 0.f;
+        float *to = scales + lane * SP;
+        *reinterpret_cast<float4 *>(to) = make_float4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<float4 *>(to + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        if (ZEROS) {
+            uint2 z = make_uint2(zn[0], zn[1]);
+            if (!full && packed && NG == 2) z = make_uint2((zn[0] & 0xffffu) | zn[1] << 16, (zn[2] & 0xffffu) | zn[3] << 16);
+            if (!packed) z = make_uint2(zn[0] | zn[1] << 8 | zn[2] << 16 | zn[3] << 24, zn[4] | zn[5] << 8 | zn[6] << 16 | zn[7] << 24);
+            *reinterpret_cast<uint2 *>(to + SG) = z;
         }
-        if (ZEROS)
-#pragma unroll
-            for (int n = 0; n < NB; n++) {
-                uint32_t z = 0;
-                if (cut.wide) z = zn[n];
-                else
-#pragma unroll
-                    for (int j = 0; j < NG; j++) z |= zn[n * NG + j] << (8 * j);
-                reinterpret_cast<uint32_t *>(to)[GU + n] = z;
-            }
     };
 
-    // ---- x: the four vectors of a lane, each loaded again for the next block as soon as it has been taken
+    // ---- x: in operand order in shared memory, put there once a CTA, or where it does not fit the four vectors of a lane from the L1, each
+    // loaded again for the next block as soon as it has been taken
     const uint8_t *const xrow = (const uint8_t *)p.x + (long)(g < p.N ? g : 0) * p.x_ld * X::SIZE;
     const int xk = g < p.N ? p.K : 0;  // (columns beyond the rows of x are zeros)
     XVec<X> xv[4];
-    auto x_at = [&](int b, int i) { return b * 128 + (i / VW) * GROUP + t * 8 * VW + (i % VW) * 8; };
+    auto x_at = [&](int b, int i, int tt) { return b * 128 + (i / VW) * GROUP + tt * 8 * VW + (i % VW) * 8; };
+    uint4 *const xs = reinterpret_cast<uint4 *>(smem + X_AT);  // [block][vector][part][N][t], then a zero for the lanes beyond the rows
+    const int xstep = g < p.N ? p.N * 4 : 0;
+    const uint4 *const xmine = g < p.N ? xs + g * 4 + t : xs + blocks * 4 * X::PARTS * p.N * 4;
 
     // The weights do not depend on the launch before this one: the first stage is under way while that one drains.
     fetch();
     fetch_scales(tile0 + mw, b0);
     pdl_enter();
+    if constexpr (XS) {
+        for (int e = tid; e < blocks * 16 * p.N; e += WARPS * 32) {
+            const int tt = e & 3, n = (e >> 2) % p.N, i = (e >> 2) / p.N & 3, b = (e >> 2) / p.N >> 2, k = x_at(b, i, tt);
+            XVec<X> v;
+            v.load((const uint8_t *)p.x + (long)n * p.x_ld * X::SIZE, k, p.K);
+            if (p.K - k > 0 && p.K - k < 8) v.cut(p.K - k);
+            uint32_t r[X::PARTS][4];
+            v.get(r);
 #pragma unroll
-    for (int i = 0; i < 4; i++) xv[i].load(xrow, x_at(b0, i), xk);
+            for (int q = 0; q < X::PARTS; q++) xs[(((b * 4 + i) * X::PARTS + q) * p.N + n) * 4 + tt] = make_uint4(r[q][0], r[q][1], r[q][2], r[q][3]);
+        }
+        if (tid == 0) xs[blocks * 4 * X::PARTS * p.N * 4] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) xv[i].load(xrow, x_at(b0, i, t), xk);
+    }
 
     // where this lane's codes of row g lie in a stage: pieces differ in bits 4 to 6 by what their number differs in
     const uint32_t lane_at = warp * STAGES * STAGE + piece(g, t * VW / 4) + t * VW % 4 * 4;
@@ -335,10 +364,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
         if (tile < tile1 && b0 < b1)
             for (int b = b0; b < b1; b += NB) {
                 __syncwarp();  // (all lanes have read the last stage and its scales)
-                put_scales(b);
+                if ((b - b0) % SB == 0) {
+                    put_scales(b);
+                    const bool wraps = b + SB >= b1;
+                    fetch_scales(wraps ? tile + wm : tile, wraps ? b0 : b + SB);
+                }
                 fetch();
-                const bool wraps = b + NB >= b1;
-                fetch_scales(wraps ? tile + wm : tile, wraps ? b0 : b + NB);
                 cp_async_wait<STAGES - 1>();
                 __syncwarp();
                 const uint32_t at = lane_at + slot * STAGE;
@@ -346,11 +377,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
 #pragma unroll
                 for (int n = 0; n < NB; n++) {
                     if (b + n >= b1) break;
-                    const int next = b + n + 1 < b1 ? b + n + 1 : b0;
-                    if ((b + n) * 128 + 128 > p.K)
+                    const int next = b + n + 1 < b1 ? b + n + 1 : b0, sb = (b - b0) % SB + n;
+                    const uint4 *const xblock = xmine + (b + n) * 4 * X::PARTS * xstep;
+                    if (!XS && (b + n) * 128 + 128 > p.K)
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const int left = p.K - x_at(b + n, i);
+                            const int left = p.K - x_at(b + n, i, t);
                             if (left > 0 && left < 8) xv[i].cut(left);
                         }
                     // the block's scales and zero points of the lane's four rows
@@ -358,14 +390,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
                     uint32_t zs[4];
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const float *from = scales + (g + 8 * r) * SP<NG>;
+                        const float *from = scales + (g + 8 * r) * SP;
                         if constexpr (NG == 4) {
-                            const float4 v = *reinterpret_cast<const float4 *>(from + n * NG);
+                            const float4 v = *reinterpret_cast<const float4 *>(from + sb * NG);
                             sc[r][0] = v.x; sc[r][1 % NG] = v.y; sc[r][2 % NG] = v.z; sc[r][3 % NG] = v.w;
                         } else
 #pragma unroll
-                            for (int j = 0; j < NG; j++) sc[r][j] = from[n * NG + j];
-                        if (ZEROS) zs[r] = reinterpret_cast<const uint32_t *>(from)[GU + n];
+                            for (int j = 0; j < NG; j++) sc[r][j] = from[sb * NG + j];
+                        if (ZEROS) zs[r] = reinterpret_cast<const uint32_t *>(from)[SG + sb * NG / 4] >> (sb * NG % 4 * 8);
                     }
 #pragma unroll
                     for (int j = 0; j < NG; j++) {
@@ -393,8 +425,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
 #pragma unroll
                         for (int h = 0; h < VW; h++) {
                             uint32_t xb[X::PARTS][4];
-                            xv[j * VW + h].get(xb);
-                            xv[j * VW + h].load(xrow, x_at(next, j * VW + h), xk);
+                            if constexpr (XS) {
+#pragma unroll
+                                for (int q = 0; q < X::PARTS; q++) {
+                                    const uint4 v = xblock[((j * VW + h) * X::PARTS + q) * xstep];
+                                    xb[q][0] = v.x; xb[q][1] = v.y; xb[q][2] = v.z; xb[q][3] = v.w;
+                                }
+                            } else {
+                                xv[j * VW + h].get(xb);
+                                xv[j * VW + h].load(xrow, x_at(next, j * VW + h, t), xk);
+                            }
 #pragma unroll
                             for (int i = 0; i < 2; i++) {
                                 uint32_t a[2][4];
@@ -459,25 +499,42 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
     cp_async_wait<0>();
 }
 
+template <typename X, int GROUP, bool ZEROS, bool XS> int launch_q4_kernel(const Q4Params &p, const Q4Cut &c, int grid, int dev, cudaStream_t st)
+{
+    const auto kern = gemv_q4_kernel<X, GROUP, ZEROS, XS>;
+    static bool set[64];
+    if (!set[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, XS ? X_AT + X_MOST : X_AT);
+        if (e != cudaSuccess) return thb_note_launch(e, "gemv_q4_kernel attributes");
+        set[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = X_AT + (XS ? (p.K + 127) / 128 * 256 * X::PARTS * p.N + 16 : 0);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = thb_pdl_enabled() ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, c);
+    return thb_note_launch(e != cudaSuccess ? e : cudaGetLastError(), "gemv_q4_kernel");
+}
+
 template <typename X, int GROUP, bool ZEROS> int launch_q4_group(const Q4Params &p, cudaStream_t st)
 {
     constexpr int NG = 128 / GROUP;
-    const auto kern = gemv_q4_kernel<X, GROUP, ZEROS>;
-    static int sms[64];
+    const int sms = thb_sm_count();
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return thb_refuse(THB_ERR_UNSUPPORTED, "thb_gemv_q4_fwd: device ordinal above 63");
-    if (!sms[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM<NG>);
-        if (e != cudaSuccess) return thb_note_launch(e, "gemv_q4_kernel attributes");
-        sms[dev] = thb_sm_count();
-    }
     Q4Cut c;
     const int blocks = (p.K + 127) / 128;
     c.tiles = (p.M + 31) / 32;
     // As few warps to a row as keep a CTA's warps equally busy: the blocks that a warp takes one after the other, and two more a tile for the
     // parts' exchange.
-    const int grid = c.tiles < sms[dev] ? c.tiles : sms[dev], most = (c.tiles + grid - 1) / grid;
+    const int grid = c.tiles < sms ? c.tiles : sms, most = (c.tiles + grid - 1) / grid;
     long best = 0;
     for (int wk = 1; wk <= WARPS && (wk == 1 || wk < 2 * blocks); wk *= 2) {
         const long steps = (most + WARPS / wk - 1) / (WARPS / wk), cost = steps * ((blocks + wk - 1) / wk + (wk > 1 ? 2 : 0));
@@ -487,20 +544,14 @@ template <typename X, int GROUP, bool ZEROS> int launch_q4_group(const Q4Params 
         }
     }
     c.mine = (blocks + c.wk - 1) / c.wk;
-    c.wide = p.s_dtype != THB_F32 && p.s_ld % NG == 0 && reinterpret_cast<uintptr_t>(p.wscale) % (2 * NG) == 0 &&
-             (!p.wzero || (p.z_ld % NG == 0 && reinterpret_cast<uintptr_t>(p.wzero) % NG == 0));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(WARPS * 32);
-    cfg.dynamicSmemBytes = SMEM<NG>;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = thb_pdl_enabled() ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, c);
-    return thb_note_launch(e != cudaSuccess ? e : cudaGetLastError(), "gemv_q4_kernel");
+    auto aligned = [&](int n) {
+        return p.s_dtype != THB_F32 && p.s_ld % n == 0 && reinterpret_cast<uintptr_t>(p.wscale) % (2 * n) == 0 &&
+               (!p.wzero || (p.z_ld % n == 0 && reinterpret_cast<uintptr_t>(p.wzero) % n == 0));
+    };
+    // (a warp's first block is a multiple of mine)
+    c.wide = aligned(SG) && (c.wk == 1 || c.mine * NG % SG == 0) ? 2 : aligned(NG) ? 1 : 0;
+    return (long)blocks * 256 * X::PARTS * p.N + 16 <= X_MOST ? launch_q4_kernel<X, GROUP, ZEROS, true>(p, c, grid, dev, st)
+                                                              : launch_q4_kernel<X, GROUP, ZEROS, false>(p, c, grid, dev, st);
 }
 
 template <typename X> int launch_q4(const Q4Params &p, int group, cudaStream_t st)
