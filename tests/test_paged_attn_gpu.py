@@ -253,3 +253,26 @@ def test_attention_streams_and_graphs(lib):
     graphs[0].replay()
     torch.cuda.synchronize()
     a.check()
+
+
+@pytest.mark.parametrize("dtype", EVERY)
+@pytest.mark.parametrize("dim", [64, 72, 96, 128, 160, 256])
+@pytest.mark.parametrize("heads,q_heads,length,window", [(1, 16, 3000, 0), (2, 48, 900, 700), (8, 8, 5000, 0), (4, 28, 260, 0), (1, 1, 16500, 16400)])
+def test_attention_one_row(lib, dtype, dim, heads, q_heads, length, window):
+    """A single row, its length shared by as many CTAs as there may be: clusters of every size, a second launch, more than eight and more
+    than sixteen heads a key head."""
+    step = Step(dtype, [length], heads, q_heads, dim, page_len=32, window=window, seed=dim)
+    assert step.call(lib) == 0, lib.thb_last_cuda_error()
+    torch.cuda.synchronize()
+    step.check()
+    assert int(step.cache.status) == 0
+
+
+@pytest.mark.parametrize("dtype", EVERY)
+@pytest.mark.parametrize("max_len", [100, 4000, 40000])
+def test_attention_rows_without_tokens(lib, dtype, max_len):
+    """Only empty and padded rows, however the call is cut: zeros, and what was there."""
+    step = Step(dtype, [0, -1, 0], 2, 4, 64, max_len=max_len, window=0)
+    assert step.call(lib) == 0
+    torch.cuda.synchronize()
+    step.check()
