@@ -150,20 +150,25 @@ template <> struct XVec<XF32> {
 #pragma unroll
         for (int i = 1; i < 8; i++) v[i] = i < left ? v[i] : 0.f;
     }
-    // A part is the top 16 bits of what the parts before it leave: 8 bits of mantissa each, no rounding, the rest is exact (that of an
-    // infinity is zero, not NaN).
+    // A part is the top 16 bits of what the parts before it leave: 8 bits of mantissa each, no rounding, the rest is exact.  (The rest of an
+    // infinity is zero, not NaN: looked at where one of the eight times zero is not zero.)
     __device__ __forceinline__ void get(uint32_t (&b)[3][4]) const
     {
         uint32_t part[3][8];
+        float zero = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) zero = fmaf(v[i], 0.f, zero);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             part[0][i] = __float_as_uint(v[i]);
 #pragma unroll
-            for (int q = 1; q < 3; q++) {
-                const float x = __uint_as_float(part[q - 1][i]), top = __uint_as_float(part[q - 1][i] & 0xffff0000u);
-                part[q][i] = __float_as_uint(x == top ? 0.f : x - top);
-            }
+            for (int q = 1; q < 3; q++)
+                part[q][i] = __float_as_uint(__uint_as_float(part[q - 1][i]) - __uint_as_float(part[q - 1][i] & 0xffff0000u));
         }
+        if (zero != 0.f)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (isinf(v[i])) part[1][i] = part[2][i] = 0;
 #pragma unroll
         for (int q = 0; q < 3; q++)
 #pragma unroll
