@@ -336,7 +336,8 @@ int thb_conv_u8_fwd_static(const thb_conv_desc *d, const void *x, void *y, thb_s
  * sum, y and q (with q_scale) are optional, one of them at least is given; the norm is taken from t before it is rounded for
  * `sum`.  sum, y may be x or res themselves.  Values behind C up to the next multiple of the alignment are ignored in x and
  * res and written as zeros.  A row whose v are all below 2^-100 has q_scale = 0 and zeros in q; one with an infinite or NaN t, or a
- * norm beyond fp32's range, has q_scale = NaN.  C <= 32768. */
+ * norm beyond fp32's range, has q_scale = NaN.  A value within 2^-22 of itself of the border between two codes may take either.
+ * C <= 32768. */
 typedef struct thb_rmsnorm_desc {
     int dtype; /* F32 / F16 / BF16: of x, res, sum, y */
     int C;
@@ -429,7 +430,8 @@ int thb_kv_append_fwd(const thb_kv_append_desc *d, const void *k, const void *v,
  * What lies behind len[r] in a page is not looked at, whatever it holds.  len[r] = 0: y is zero, lse -infinity; len[r] < 0: a place in a
  * padded batch, whose row of y and lse stays as it is.  A length above max_len or the table is cut to it, a position whose page is not
  * of the pool left out, a sequence that does not exist taken as empty; *status becomes THB_ERR_ARG.  max_len decides how a row is split among CTAs, and so the
- * order of its sums; scratch is for the parts of one call at a time (thb_paged_attn_scratch bytes, 0: none is needed). */
+ * order of its sums; scratch (16-byte aligned) is for the parts of one call at a time (thb_paged_attn_scratch bytes, 0: none is needed).
+ * rows <= 65535. */
 typedef struct thb_paged_attn_desc {
     thb_kv_cache cache;
     int rows, q_heads, q_ld, y_ld;

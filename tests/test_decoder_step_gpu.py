@@ -154,3 +154,32 @@ def test_decoder_token_by_token(lib, dtype, codes_between):
     e = 18 * UNIT[dtype]
     limit = e if not codes_between else e + 4 * math.sqrt(8 * e) / 8
     assert float((got - ref).norm() / ref.norm()) < limit
+
+
+def first_calls_captured():
+    """(in a process of its own)"""
+    lib = K.load()
+    for dtype, codes_between in ((K.THB_F16, True), (K.THB_F32, False)):
+        captured, eager = Decoder(lib, dtype, codes_between), Decoder(lib, dtype, codes_between)
+        for dec in (captured, eager):
+            dec.x.copy_(torch.randn(SEQS, WIDTH, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)))
+            dec.len.fill_(1)
+        torch.cuda.synchronize()
+        s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            captured.step(s.cuda_stream)
+        graph.replay()
+        eager.step(None)
+        torch.cuda.synchronize()
+        assert torch.equal(captured.stream_sum, eager.stream_sum) and bool((eager.stream_sum != 0).any())
+
+
+def test_first_calls_of_a_process_captured():
+    """Nothing that a first call sets up has to happen outside of a capture."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = "import sys; sys.path[:0] = [%r, %r]; import test_decoder_step_gpu as t; t.first_calls_captured()" % (here, os.path.dirname(here))
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
