@@ -167,3 +167,25 @@ def test_gemv_q4_of_quantized_weights(lib):
     torch.cuda.synchronize()
     ref, size = layer.sums()
     check(layer, ref, layer.off() * size)
+
+
+def test_gemv_q4_offsets_beyond_32_bits(lib):
+    """More than 2^32 bytes of codes: the first, some middle and the last rows."""
+    k, m, group = 32768, (1 << 32) // 16384 + 77, 128
+    if torch.cuda.mem_get_info()[0] < 2 * m * k:
+        pytest.skip("the device has no room for the weights")
+    w = torch.zeros(m, k // 2, device="cuda", dtype=torch.uint8)
+    some = torch.tensor([0, 31, 32, m // 2, m - 78, m - 33, m - 1], device="cuda")
+    w[some] = torch.randint(0, 256, (7, k // 2), device="cuda", dtype=torch.uint8)
+    s = torch.full((m, k // group), 0.01, device="cuda", dtype=torch.float16)
+    x = torch.randn(2, k, device="cuda").half()
+    y = torch.zeros(2, up(m, 8), device="cuda", dtype=torch.float16)
+    d = K.GemvQ4Desc(dtype=K.THB_F16, N=2, K=k, M=m, group=group, x_ld=k, y_ld=y.stride(0), w_ld=k // 2, s_ld=k // group, wscale_dtype=K.THB_F16,
+                     w=w.data_ptr(), wscale=s.data_ptr())
+    assert lib.thb_gemv_q4_fwd(C.byref(d), x.data_ptr(), None, y.data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    codes = torch.stack((w[some] & 15, w[some] >> 4), 2).reshape(7, k).double() - 8
+    ws = codes * s[some].double().repeat_interleave(group, 1)
+    ref, size = x.double() @ ws.T, x.double().abs() @ ws.abs().T
+    bound = (17 * 8 * 2.0 ** -23 + (4 * (k / 1024 + 1) + 12) * 2.0 ** -24) * size + UNIT[K.THB_F16] * ref.abs()
+    assert bool(((y[:, some].double() - ref).abs() <= bound).all())

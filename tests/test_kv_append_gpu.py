@@ -104,7 +104,8 @@ def run(lib, dtype, heads, q_heads, dim, page_len, seqs, a_seq, pos, seq, rot, i
 @pytest.mark.parametrize("dtype", EVERY)
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("heads,q_heads,dim,rot", [(1, 1, 8, 8), (2, 6, 64, 64), (3, 3, 80, 40), (8, 32, 128, 128), (1, 5, 96, 6), (2, 2, 128, 24),
-                                                   (4, 4, 256, 256), (2, 4, 64, 0), (1, 2, 40, 2)])
+                                                   (4, 4, 256, 256), (2, 4, 64, 0), (1, 2, 40, 2), (1, 2, 256, 0), (2, 3, 256, 64), (2, 2, 80, 20), (1, 40, 256, 6),
+                                                   (20, 20, 32, 32)])
 def test_append_heads_and_rotations(lib, dtype, interleaved, heads, q_heads, dim, rot):
     run(lib, dtype, heads, q_heads, dim, 16, 3, 4, pos=[0, 17, 63], seq=None, rot=rot, interleaved=interleaved, by_head=rot % 3 == 0)
 

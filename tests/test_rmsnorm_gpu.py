@@ -139,3 +139,19 @@ def test_rmsnorm_empty_and_streams(lib):
     s.synchronize()
     t, v = formula(x, None, None, 1e-5)
     check(K.THB_F16, 512, t, v, None, y, None, None)
+
+
+def test_rmsnorm_offsets_beyond_32_bits(lib):
+    """More than 2^32 values: the first and the last rows."""
+    rows, c = (1 << 32) // 4096 + 5, 4096
+    if torch.cuda.mem_get_info()[0] < 6 * rows * c:
+        pytest.skip("the device has no room for the rows")
+    x = torch.zeros(rows, c, device="cuda", dtype=torch.float16)
+    ends = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1], device="cuda")
+    x[ends] = torch.randn(5, c, device="cuda").half()
+    y = torch.full_like(x, 7.0)
+    assert call(lib, K.THB_F16, c, x, y=y) == 0
+    torch.cuda.synchronize()
+    t, v = formula(x[ends], None, None, 1e-5)
+    check(K.THB_F16, c, t, v, None, y[ends], None, None)
+    assert bool((y[2:1000] == 0).all()) and bool((y[rows - 1000:rows - 2] == 0).all())
