@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
     const int xstep = g < p.N ? p.N * 4 : 0;
     const uint4 *const xmine = g < p.N ? xs + g * 4 + t : xs + blocks * 4 * X::PARTS * p.N * 4;
 
-    // The weights do not depend on the launch before this one: the first stage is under way while that one drains.
+    // The weights do not depend on the launch before this one: the first stage is under way while that one drains (a chain of 4096->4096 fp16 on one
+    // row from HBM 5.9 -> 5.3 us a call, 9216->4096 bf16 on eight 12.1 -> 11.0; brought as far as the L2 only: no gain).
     fetch();
     fetch_scales(tile0 + mw, b0);
     pdl_enter();
