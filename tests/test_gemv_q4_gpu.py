@@ -189,3 +189,25 @@ def test_gemv_q4_offsets_beyond_32_bits(lib):
     ref, size = x.double() @ ws.T, x.double().abs() @ ws.abs().T
     bound = (17 * 8 * 2.0 ** -23 + (4 * (k / 1024 + 1) + 12) * 2.0 ** -24) * size + UNIT[K.THB_F16] * ref.abs()
     assert bool(((y[:, some].double() - ref).abs() <= bound).all())
+
+
+def test_gemv_q4_of_weights_just_written(lib):
+    """Codes, scales and zero points that the launch before in the stream writes, over and over: each product is of its own."""
+    layer = Layer(K.THB_F16, 2, 4096, 2048, 64)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    sets = [(torch.randint(0, 256, layer.w.shape, device="cuda", generator=g, dtype=torch.uint8), torch.rand(layer.s.shape, device="cuda", generator=g).half(),
+             torch.randint(0, 16, layer.z.shape, device="cuda", generator=g, dtype=torch.uint8)) for _ in range(3)]
+    got = []
+    for i in range(60):
+        layer.z.copy_(sets[i % 3][2]), layer.s.copy_(sets[i % 3][1]), torch.bitwise_or(sets[i % 3][0], 0, out=layer.w)
+        assert layer.call(lib, torch.cuda.current_stream().cuda_stream) == 0
+        got.append(layer.y.clone())
+    torch.cuda.synchronize()
+    for i in range(57):
+        assert torch.equal(got[i], got[i + 3])
+    for i in range(3):
+        for t, src in zip((layer.w, layer.s, layer.z), sets[i]):
+            t.copy_(src)
+        layer.y.copy_(got[i])
+        ref, size = layer.sums()
+        check(layer, ref, layer.off() * size)
