@@ -45,6 +45,23 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// c = a b: a group's first product
+template <bool BF>
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    if (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// 8 rows of 16 bytes four times: lane (g, t) gets word t of rows g, g + 8, g + 16 and g + 24, whose addresses lanes 0 to 31 give
+__device__ __forceinline__ void codes_of(uint32_t (&w)[4], uint32_t at)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+}
+
 // (a & mask) | base in one instruction
 __device__ __forceinline__ uint32_t code_pair(uint32_t a, uint32_t mask, uint32_t base)
 {
@@ -52,8 +69,8 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t a, uint32_t mask, uint32_
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(base));
     return d;
 }
-// the zero point of a row's group as what is subtracted from a pair: z + 1024 (fp16) or z + 128 (bf16) twice
-template <bool BF> __device__ __forceinline__ uint32_t zero_pair(uint32_t z) { return ((z & 15) | (BF ? 0x4300u : 0x6400u)) * 0x10001u; }
+// the zero point of a row's group (byte i of four) as what is subtracted from a pair: z + 1024 (fp16) or z + 128 (bf16) twice
+template <bool BF> __device__ __forceinline__ uint32_t zero_pair(uint32_t z, int i) { return __byte_perm(z, BF ? 0x43u : 0x64u, 0x4040 + i * 0x0101); }
 // codes (0, 4), (1, 5), (2, 6), (3, 7) of a word (nibbles, lowest first) less the zero point, as pairs of 16-bit numbers.  In fp16 the odd
 // ones are taken where they stand, as 1024 + 16 q, and scaled by the subtraction of 64 + z.
 template <bool BF> __device__ __forceinline__ void pairs_of(uint32_t word, uint32_t za, uint32_t zb, uint32_t (&d)[4])
@@ -191,12 +208,15 @@ constexpr int X_AT = SCALES_AT + WARPS * 32 * SP * 4, X_MOST = 227 * 1024 - 1024
 // blocks a stage, by cp.async of 16 bytes (no registers, no barrier between warps: 64 KB under way an SM while as much is multiplied).  x comes
 // from the L1, a block ahead, and each of its operands is multiplied by both 16-row halves of the tile.  Where the tiles are too few for the
 // warps, wk of them share a row's blocks and their parts are added through shared memory; else a warp has whole rows.
-// Lane (g = lane / 4, t = lane % 4) holds rows g, g + 8, g + 16 and g + 24.  Of a block it takes the k of its t: 32 in one vector where a group
-// is 128 long, 16 of each of two groups, 8 of each of four, so that a product's k are all of one group.
+// Lane (g = lane / 4, t = lane % 4) holds rows g, g + 8, g + 16 and g + 24.  Of each 32 k it takes the 8 of its t, word t of 16 bytes: what ldmatrix
+// gives it of four times eight rows.
 template <typename X, int GROUP, bool ZEROS, bool XS>
 __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cut cut)
 {
-    constexpr int VW = GROUP / 32, NG = 128 / GROUP, SB = SG / NG;  // words a load, groups a block, blocks whose scales are at hand
+    constexpr int VW = GROUP / 32, NG = 128 / GROUP, SB = SG / NG;  // words of a lane's row a group, groups a block, blocks whose scales are at hand
+    // A block's codes are read at once where x comes from the L1 (11008->11000 on four rows 27.5 -> 25.0 us) or a group is a block (4096->128000
+    // 54.5 -> 53.9); else as they are needed, for the registers' sake (4096->32003 in e4m3, groups of 32, 28.8 -> 28.3).
+    constexpr bool AHEAD = !XS || NG == 1;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t ring = smem_u32(smem) + warp * STAGES * STAGE;
@@ -205,8 +225,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
     const int blocks = (p.K + 127) / 128, groups = (p.K + GROUP - 1) / GROUP, bytes = ((p.K + 1) / 2 + 15) / 16 * 16;
     const int b0 = kw * cut.mine, b1 = min(blocks, b0 + cut.mine);  // (b0 may be beyond the row: then there is nothing to add)
 
-    // 16-byte pieces of a stage, permuted so that no load of 8, 4 or 2 rows meets a bank twice
-    auto piece = [](int row, int c) { return ((row * 8 + c) ^ (VW == 4 ? (row & 1) << 2 : VW == 2 ? (row & 3) << 1 : row & 7)) * 16; };
+    // 16-byte pieces of a stage, permuted so that no load of 8 rows meets a bank twice
+    auto piece = [](int row, int c) { return ((row * 8 + c) ^ (row & 7)) * 16; };
 
     // ---- the codes' loads, a stage ahead of the products; lane: pieces fc of rows fr, fr + 4, ...
     const int fr = lane >> 3, fc = lane & 7;
@@ -320,7 +340,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
             uint2 z = make_uint2(zn[0], zn[1]);
             if (!full && packed && NG == 2) z = make_uint2((zn[0] & 0xffffu) | zn[1] << 16, (zn[2] & 0xffffu) | zn[3] << 16);
             if (!packed) z = make_uint2(zn[0] | zn[1] << 8 | zn[2] << 16 | zn[3] << 24, zn[4] | zn[5] << 8 | zn[6] << 16 | zn[7] << 24);
-            *reinterpret_cast<uint2 *>(to + SG) = z;
+            *reinterpret_cast<uint2 *>(to + SG) = make_uint2(z.x & 0x0f0f0f0fu, z.y & 0x0f0f0f0fu);
         }
     };
 
@@ -329,7 +349,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
     const uint8_t *const xrow = (const uint8_t *)p.x + (long)(g < p.N ? g : 0) * p.x_ld * X::SIZE;
     const int xk = g < p.N ? p.K : 0;  // (columns beyond the rows of x are zeros)
     XVec<X> xv[4];
-    auto x_at = [&](int b, int i, int tt) { return b * 128 + (i / VW) * GROUP + tt * 8 * VW + (i % VW) * 8; };
+    auto x_at = [&](int b, int i, int tt) { return b * 128 + i * 32 + tt * 8; };
     uint4 *const xs = reinterpret_cast<uint4 *>(smem + X_AT);  // [block][vector][part][N][t], then a zero for the lanes beyond the rows
     const int xstep = g < p.N ? p.N * 4 : 0;
     const uint4 *const xmine = g < p.N ? xs + g * 4 + t : xs + blocks * 4 * X::PARTS * p.N * 4;
@@ -357,8 +377,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
         for (int i = 0; i < 4; i++) xv[i].load(xrow, x_at(b0, i, t), xk);
     }
 
-    // where this lane's codes of row g lie in a stage: pieces differ in bits 4 to 6 by what their number differs in
-    const uint32_t lane_at = warp * STAGES * STAGE + piece(g, t * VW / 4) + t * VW % 4 * 4;
+    // where row `lane` lies in a stage: pieces differ in bits 4 to 6 by what their number differs in
+    const uint32_t lane_at = ring + piece(lane, 0);
     int slot = 0;
     for (int step = tile0; step < tile1; step += wm) {
         const int tile = step + mw;
@@ -391,6 +411,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
                             const int left = p.K - x_at(b + n, i, t);
                             if (left > 0 && left < 8) xv[i].cut(left);
                         }
+                    uint32_t w[4][4];
+                    if (AHEAD)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) codes_of(w[i], at ^ (n * 4 + i) * 16);
                     // the block's scales and zero points of the lane's four rows
                     float sc[4][NG];
                     uint32_t zs[4];
@@ -403,34 +427,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
                         } else
 #pragma unroll
                             for (int j = 0; j < NG; j++) sc[r][j] = from[sb * NG + j];
-                        if (ZEROS) zs[r] = reinterpret_cast<const uint32_t *>(from)[SG + sb * NG / 4] >> (sb * NG % 4 * 8);
+                        if (ZEROS) zs[r] = reinterpret_cast<const uint32_t *>(from)[SG + sb * NG / 4];
                     }
 #pragma unroll
                     for (int j = 0; j < NG; j++) {
                         float c[2][4];
-                        uint32_t w[4][VW], za[4], zb[4];
-                        const int c0 = n * 4 + j * (GROUP / 32);
-#pragma unroll
-                        for (int i = 0; i < 2; i++)
-#pragma unroll
-                            for (int q = 0; q < 4; q++) c[i][q] = 0.f;
+                        uint32_t za[4], zb[4];
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
-                            const uint8_t *src = smem + (at ^ c0 * 16) + r * 1024;
-                            if constexpr (VW == 4) {
-                                const uint4 v = *reinterpret_cast<const uint4 *>(src);
-                                w[r][0] = v.x; w[r][1 % VW] = v.y; w[r][2 % VW] = v.z; w[r][3 % VW] = v.w;
-                            } else if constexpr (VW == 2) {
-                                const uint2 v = *reinterpret_cast<const uint2 *>(src);
-                                w[r][0] = v.x; w[r][1 % VW] = v.y;
-                            } else
-                                w[r][0] = *reinterpret_cast<const uint32_t *>(src);
-                            za[r] = zero_pair<X::BF>(ZEROS ? zs[r] >> (8 * j) : 8);
+                            za[r] = ZEROS ? zero_pair<X::BF>(zs[r], sb * NG % 4 + j) : X::BF ? 0x43084308u : 0x64086408u;
                             zb[r] = X::BF ? 0 : zero_pair_16(za[r]);
                         }
 #pragma unroll
                         for (int h = 0; h < VW; h++) {
                             uint32_t xb[X::PARTS][4];
+                            if (!AHEAD) codes_of(w[j * VW + h], at ^ (n * 4 + j * VW + h) * 16);
                             if constexpr (XS) {
 #pragma unroll
                                 for (int q = 0; q < X::PARTS; q++) {
@@ -445,10 +456,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
                             for (int i = 0; i < 2; i++) {
                                 uint32_t a[2][4];
 #pragma unroll
-                                for (int r = 0; r < 2; r++) pairs_of<X::BF>(w[2 * i + r][h], za[2 * i + r], zb[2 * i + r], a[r]);
+                                for (int r = 0; r < 2; r++) pairs_of<X::BF>(w[j * VW + h][2 * i + r], za[2 * i + r], zb[2 * i + r], a[r]);
 #pragma unroll
                                 for (int q = X::PARTS - 1; q >= 0; q--) {
-                                    mma16816<X::BF>(c[i], a[0][0], a[1][0], a[0][1], a[1][1], xb[q][0], xb[q][1]);
+                                    if (h == 0 && q == X::PARTS - 1) mma16816_first<X::BF>(c[i], a[0][0], a[1][0], a[0][1], a[1][1], xb[q][0], xb[q][1]);
+                                    else mma16816<X::BF>(c[i], a[0][0], a[1][0], a[0][1], a[1][1], xb[q][0], xb[q][1]);
                                     mma16816<X::BF>(c[i], a[0][2], a[1][2], a[0][3], a[1][3], xb[q][2], xb[q][3]);
                                 }
                             }
