@@ -7,12 +7,13 @@
 // A code becomes q - z in 16 bits exactly (an integer of 5 bits): or'ed into the mantissa of 1024 (fp16; bf16: 128), then z + 1024 is
 // subtracted.  Products and their sums are exact or fp32, a group's sum takes its scale in fp32.  x in fp32 is three bf16 parts
 // (8 + 8 + 8 bits), each multiplied; e4m3 codes are fp16 numbers.
-// What bounds it: the instructions a weight takes, 9 (fp16) or 11 (bf16) for 8 weights to unpack them, as many again for everything else; the
-// half-rate integer pipe is the busiest.  us a call in a chain (of the measured copy rate): 4096->128000, one row, bf16 groups of 128 53.9
-// (5.0 TB/s, 77 %); 4096->32003, four rows of e4m3, groups of 32 23.7 (48 %); 14336->4096, one row, fp16 10.2 (46 %); 9216->4096, eight rows,
-// bf16 groups of 64 with zero points 10.3 (31 %); 25088->4096, three rows, fp32 39 (21 %: 300 of its instructions a block take x apart).
-// Before: codes straight from global memory into registers 164 us for the 4096->32003, x in registers and tiles of 16 rows 31, x from
-// the L1 27.
+// What bounds it: 9 (fp16) or 11 (bf16) instructions unpack 8 weights, as many again do everything else, and sixteen warps of 128 registers
+// issue in 40 to 55 % of the cycles only (waits for a stage, for shared memory, for warps with a tile more).  us a call in a chain (of the measured copy rate): 4096->128000, one row, bf16 groups of 128 53.9
+// (5.0 TB/s, 77 %); 4096->32003, four rows of e4m3, groups of 32 28.2 (43 %); 14336->4096, one row, fp16 11.4 (41 %); 9216->4096, eight rows,
+// bf16 groups of 64 with zero points 10.4 (31 %); 25088->4096, three rows, fp32 32.3 (25 %: most of its instructions take x apart).
+// Before: codes straight from global memory into registers 164 us for the 4096->32003, x in registers and tiles of 16 rows 31.  Tried and
+// slower: an equal share of a CTA's blocks for each warp, across tiles (a block or two less a warp, but 0.2 to 4 us more a call for where parts
+// begin and how they are joined); fp32 vectors taken apart by a warp's lanes together and handed on through shared memory (36 for 32).
 #include "tokens.cuh"
 #include <cuda_fp8.h>
 
@@ -206,8 +207,8 @@ constexpr int X_AT = SCALES_AT + WARPS * 32 * SP * 4, X_MOST = 227 * 1024 - 1024
 
 // One CTA of sixteen warps to an SM owns a range of tiles.  The codes come through a ring of a warp's own in shared memory, 32 rows by two
 // blocks a stage, by cp.async of 16 bytes (no registers, no barrier between warps: 64 KB under way an SM while as much is multiplied).  x comes
-// from the L1, a block ahead, and each of its operands is multiplied by both 16-row halves of the tile.  Where the tiles are too few for the
-// warps, wk of them share a row's blocks and their parts are added through shared memory; else a warp has whole rows.
+// in operand order from shared memory, or where it does not fit from the L1, a block ahead, and each of its operands is multiplied by both
+// 16-row halves of the tile.  Where the tiles are too few for the warps, wk of them share a row's blocks and their parts are added through shared memory; else a warp has whole rows.
 // Lane (g = lane / 4, t = lane % 4) holds rows g, g + 8, g + 16 and g + 24.  Of each 32 k it takes the 8 of its t, word t of 16 bytes: what ldmatrix
 // gives it of four times eight rows.
 template <typename X, int GROUP, bool ZEROS, bool XS>
