@@ -4,8 +4,8 @@
 // pos * freq in fp32 is off by 0.06 rad at a million positions, so the angle is reduced to a fraction of a turn in fp64, once a pair and
 // token for all its heads, and cos and sin are taken of that in fp32.  HBM-bound on prompts (each value read and written once),
 // latency-bound on a decoder's single tokens.
-// us a launch in a chain (share of the measured copy rate), 8192 tokens of 32 + 8 + 8 heads: of 128 in bf16, halves 41.0 (75 %); half of each
-// turned in neighbouring pairs, fp16 41.7 (74 %); of 64 26.7 (58 %); 4096 tokens in fp32 37.1 (83 %).  With a block to a token, which
+// us a launch in a chain (share of the measured copy rate), 8192 tokens of 32 + 8 + 8 heads: of 128 in bf16, halves 36.6 (84 %); half of each
+// turned in neighbouring pairs, fp16 37.5 (82 %); of 64 23.3 (66 %); 4096 tokens in fp32 34.7 (89 %).  With a block to a token, which
 // waits for the angles together: 56 / 47 / 34 / 36.
 #include "tokens.cuh"
 #include <math.h>
@@ -21,22 +21,27 @@ struct AppendParams {
     int tokens, q_heads, k_ld, v_ld, q_ld, q_out_ld;
 };
 
-// what a lane moves at a time: 16 bytes where halves and parts of a head allow, else 8, 4 or one value
-template <typename T, int U> struct alignas(sizeof(T) * U) Unit {
-    T v[U];
+// what a lane moves at a time: 16 bytes where halves and parts of a head allow, else 8, 4 or one value; held as words, so that it is one load
+template <int BYTES> struct WordOf;
+template <> struct WordOf<16> { using type = uint4; };
+template <> struct WordOf<8> { using type = uint2; };
+template <> struct WordOf<4> { using type = uint32_t; };
+template <> struct WordOf<2> { using type = uint16_t; };
+template <typename T, int U> struct Unit {
+    typename WordOf<sizeof(T) * U>::type w;
     __device__ __forceinline__ void unpack(float *f) const
     {
-        if constexpr (sizeof(T) * U == 16) Vec16<T>::unpack(*reinterpret_cast<const uint4 *>(v), f);
+        if constexpr (sizeof(T) * U == 16) Vec16<T>::unpack(w, f);
         else
 #pragma unroll
-            for (int i = 0; i < U; i++) f[i] = dt<T>::ld(v + i);
+            for (int i = 0; i < U; i++) f[i] = dt<T>::ld(reinterpret_cast<const T *>(&w) + i);
     }
     __device__ __forceinline__ void pack(const float *f)
     {
-        if constexpr (sizeof(T) * U == 16) *reinterpret_cast<uint4 *>(v) = Vec16<T>::pack(f);
+        if constexpr (sizeof(T) * U == 16) w = Vec16<T>::pack(f);
         else
 #pragma unroll
-            for (int i = 0; i < U; i++) dt<T>::st(v + i, f[i]);
+            for (int i = 0; i < U; i++) dt<T>::st(reinterpret_cast<T *>(&w) + i, f[i]);
     }
 };
 
@@ -44,10 +49,18 @@ template <typename T, int U> struct alignas(sizeof(T) * U) Unit {
 // are taken once, where there are few several share them.  A lane has the same item of each of its heads: a pair of units of both halves, a
 // unit of neighbouring pairs, or units that are not turned; the angles it turns by stay in its registers.  HEADS of them are under way, the
 // first before the position and the page are known.
+// How many heads, and blocks an SM.  Halves in whole units: few warps with many loads each (8192 tokens of 32 + 8 + 8 heads of 128 in bf16, 6 and
+// two blocks against 4 and two: 36.6 us for 39.8).  Pairs, or smaller units, take more instructions a byte: fewer loads, more warps (half of each
+// head in pairs, fp16, 3 and four against 4 and three: 37.5 for 40.3; 4096 tokens of 36 heads of 80 in units of 8 bytes, 2 and four against 4 and
+// three: 22.0 for 35.7; of single values it loses, 56.6 for 51).
+template <typename T, int U, bool INTER> struct AppendShape {
+    static constexpr bool MANY = !INTER && sizeof(T) * U == 16;
+    static constexpr int HEADS = INTER ? 3 : MANY ? 6 : 2, BLOCKS = MANY ? 2 : 4;
+};
 template <typename T, int U, bool INTER>
-__global__ void __launch_bounds__(256) kv_append_kernel(AppendParams p, int items, int per, int slots, int parts)
+__global__ void __launch_bounds__(256, (AppendShape<T, U, INTER>::BLOCKS)) kv_append_kernel(AppendParams p, int items, int per, int slots, int parts)
 {
-    constexpr int HEADS = 4, PAIRS = U == 1 ? 1 : INTER ? U / 2 : U;  // pairs an item
+    constexpr int HEADS = AppendShape<T, U, INTER>::HEADS, PAIRS = U == 1 ? 1 : INTER ? U / 2 : U;  // pairs an item
     __shared__ float2 turns_of[8][128];
     pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
