@@ -3,8 +3,10 @@
 // One pass: a row's t stay in registers between the reduction and the results.  r is common to a row, so max|v| = r * max|t * gain|
 // and the codes are e4m3(t * gain * (448 / max|t * gain|)): the sum of squares and the maximum are reduced together, and r's
 // rounding does not reach the codes.  HBM-bound on many rows, and near it by the instructions a value takes; latency-bound on few.
-// us a launch in a chain (share of the measured copy rate): 8192 rows of 4096 in fp16 with residual 43.6 (94 %), to e4m3 41.4 (87 %), without
-// residual 26.9 (76 %); 4096 of 8192 42.8 (96 %); 2048 of 16384 60 (68 %); 262144 of 128 30.6 (67 %); 8192 of 4096 in fp32 90 (91 %).
+// us a launch in a chain (share of the measured copy rate): 8192 rows of 4096 in fp16 with residual 43.3 (95 %), without residual 26.9 (76 %);
+// 4096 of 8192 42.8 (96 %); 2048 of 16384 60 (68 %); 262144 of 128 30.6 (67 %); 8192 of 4096 in fp32 90 (91 %).  To e4m3, whose codes are
+// settled as below: 8192 of 4096 in bf16 with residual 58.6 (61 %; 41.0 with codes that the roundings of fp32 decide), fp32 81.0 (82 %, 76.9),
+// without residual 44.7 (34 %, 33.1), 262144 of 128 without 41.2 (38 %, 32.1), 2048 of 16384 79 (45 %, 55.2), 1024 of 32768 in fp32 160 (42 %, 138).
 #include "tokens.cuh"
 #include <cuda_fp8.h>
 
@@ -28,12 +30,26 @@ __device__ __forceinline__ float max_nan(float a, float b)
     return r;
 }
 
+// Codes are what the formula gives in exact arithmetic, rounded to fp32 and that to e4m3.  t * gain * (448 / max) in fp32 is off by 7 units of
+// 2^-24 of itself at most (t, its product, the maximum (two), the quotient, EDGE's product, the last one), EDGE is eight: where the codes
+// of a little less and of a little more agree they are the code.  For the others, one value in a hundred thousand, fp64 leaves t's and the
+// maximum's roundings (three units; without a residual one, the maximum's); what that does not settle takes the row's maximum in exact
+// arithmetic, for which its threads come together once more.  Half of what it costs is the instructions of every row and the barrier that asks
+// whether any code is open, half the rows with such a value, 1 to 3 us each, of which one CTA has more than the others.  Tried and slower
+// (8192 of 4096 in bf16): the exact maximum of every row ahead of its first barrier 66 us; all that is rare out of line 124 (its calls spill the
+// row's registers); x and res kept in the ring until the row is done 68; rows with such values left for the end of the launch 61 (16384: 125).
+constexpr float EDGE = 8 * 0x1p-24f;
+// below this maximum 448 / max or the products leave fp32's range: all of the row's codes are settled in fp64
+constexpr float LEAST = 0x1p-100f;
+
+__device__ __forceinline__ uint32_t e4m3_of(double v) { return __nv_cvt_float_to_fp8((float)v, __NV_SATFINITE, __NV_E4M3); }
+
 // WARP: groups of `lanes` threads (a power of two up to a warp) have a row each; otherwise the whole block shares one.
 // A thread owns vectors tid, tid + threads, ... of its row, VPT at most.  Blocks stay for many rows.  Q: codes are wanted, and with them
 // the row's maximum.
 // What a block reads next is under way while a row is reduced and written: short rows' vectors in registers, longer ones' in a ring of
 // STAGES rows in shared memory by cp.async, of which every thread reads only what it asked for itself, so that nobody waits for another.
-// The gain is in registers where a thread has one vector of it, else in shared memory where that has room.
+// The gain is in registers where a thread has one or two vectors of it, else in shared memory where that has room.
 template <typename T, int VPT, bool WARP> struct NormShape {
     static constexpr int VN = Vec16<T>::N;
     static constexpr int STAGES = WARP ? 0 : VPT <= 4 ? 2 : VPT == 8 ? 1 : 0;
@@ -44,12 +60,13 @@ template <typename T, int VPT, bool WARP> struct NormShape {
     }
 };
 template <typename T, int VPT, bool WARP, bool Q>
-__global__ void __launch_bounds__(WARP ? 256 : 512) rmsnorm_kernel(NormParams p, int lanes)
+__global__ void __launch_bounds__(WARP ? 256 : 512, !Q ? 0 : WARP ? 4 : VPT <= 2 ? 2 : 1) rmsnorm_kernel(NormParams p, int lanes)
 {
     using S = NormShape<T, VPT, WARP>;
     constexpr int VN = S::VN, STAGES = S::STAGES;
     constexpr bool KEEP = S::KEEP;
     __shared__ float2 part[2][16];
+    __shared__ unsigned long long largest;
     extern __shared__ uint4 smem[];
     const int threads = WARP ? lanes : blockDim.x, tid = WARP ? threadIdx.x % lanes : threadIdx.x;
     const int per_block = WARP ? blockDim.x / lanes : 1;
@@ -147,7 +164,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) rmsnorm_kernel(NormParams p,
 #pragma unroll
                     for (int j = 0; j < VN; j++) most = max_nan(most, fabsf(t[i][j] * g[j]));
                 }
-                if (p.sum) *reinterpret_cast<uint4 *>((T *)p.sum + row * p.sum_ld + v * VN) = Vec16<T>::pack(t[i]);
+                if (!Q && p.sum) *reinterpret_cast<uint4 *>((T *)p.sum + row * p.sum_ld + v * VN) = Vec16<T>::pack(t[i]);
             } else {
 #pragma unroll
                 for (int j = 0; j < VN; j++) t[i][j] = 0.f;
@@ -159,6 +176,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) rmsnorm_kernel(NormParams p,
             slot = slot + 1 == STAGES ? 0 : slot + 1;
         }
         const int width = WARP ? lanes : 32;
+        const float own = most;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             if (o >= width) continue;
@@ -180,39 +198,125 @@ __global__ void __launch_bounds__(WARP ? 256 : 512) rmsnorm_kernel(NormParams p,
             parity ^= 1;  // (the buffers alternate, so that one barrier a row is enough)
         }
         const float r = rsqrtf(square * inv_c + p.eps);
-        float code = 0.f;
         if (Q) {
-            float scale = 0.f;
+            float scale = 0.f, code = 0.f;
+            bool all = false;
             const float top = r * most;
             if (!isfinite(square) || !isfinite(top)) scale = __int_as_float(0x7fc00000);
             else if (top >= 0x1p-100f) {
                 scale = top / 448.f;
-                code = 448.f / most;
+                all = most < LEAST;
+                if (!all) code = 448.f / most;
             }
             if (live && tid == 0) p.q_scale[row] = scale;
+            const float up = code * (1.f + EDGE), down = code * (1.f - EDGE);
+            unsigned long long marks = 0;  // of this thread's values: those that are not settled
+#pragma unroll
+            for (int i = 0; i < VPT; i++) {
+                const int v = tid + i * threads;
+                if (!live || v >= nvq) continue;
+                float g[VN];
+                gain_of(i, v, g);
+                uint32_t c[VN / 4], differs[VN / 4], apart = 0;
+#pragma unroll
+                for (int j = 0; j < VN; j += 4) {
+                    float w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) w[k] = t[i][j + k] * g[j + k];
+                    auto codes = [&](float by) {
+                        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(w[0] * by, w[1] * by), __NV_SATFINITE, __NV_E4M3);
+                        return lo | (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(w[2] * by, w[3] * by), __NV_SATFINITE, __NV_E4M3) << 16;
+                    };
+                    c[j / 4] = codes(up);
+                    apart |= differs[j / 4] = c[j / 4] ^ codes(down);
+                }
+                uint8_t *at = p.q + row * p.q_ld + v * VN;
+                if (VN == 4) *reinterpret_cast<uint32_t *>(at) = c[0];
+                else *reinterpret_cast<uint2 *>(at) = make_uint2(c[0], c[VN / 4 - 1]);
+                if (apart || all)
+#pragma unroll
+                    for (int j = 0; j < VN; j++)
+                        if (v * VN + j < p.C && (all || differs[j / 4] >> 8 * (j % 4) & 0xff)) marks |= 1ull << (i * VN + j);
+            }
+            // one marked value after the other (most often there is one): `settled` stores its code or leaves it
+            auto each = [&](unsigned long long left, auto settled) {
+#pragma unroll 1
+                for (; left; left &= left - 1) {
+                    const int at = __ffsll((long long)left) - 1, e = (tid + at / VN * threads) * VN + at % VN;
+                    if (settled(at, e, p.gain ? p.gain[e] : 1.f)) marks &= ~(1ull << at);
+                }
+            };
+            if (marks && !all) {
+                const double by = (double)code + (448. - (double)code * (double)most) * ((double)code * (1. / 448.)), off = (p.res ? 3.01 : 1.01) * 0x1p-24;
+                each(marks, [&](int at, int e, float g) {
+                    float a = 0.f;
+#pragma unroll
+                    for (int i = 0; i < VPT * VN; i++) a = i == at ? t[i / VN][i % VN] : a;
+                    const double w = (double)a * (double)g * by;
+                    const uint32_t q = e4m3_of(w * (1. + off));
+                    if (q != e4m3_of(w * (1. - off))) return false;
+                    p.q[row * p.q_ld + e] = (uint8_t)q;
+                    return true;
+                });
+            }
+            bool any;
+            if (WARP) any = __any_sync(0xffffffffu, marks != 0);
+            else {
+                if (tid == 0) largest = 0;  // (who read it for the row before has passed this row's first barrier since)
+                any = __syncthreads_or(marks != 0);
+            }
+            if (any) {
+                // (sum and y, which may take the place of x and res, are not written yet)
+                auto exact_of = [&](int e, float g) {
+                    const double x = dt<T>::ld((const T *)p.x + row * p.x_ld + e), res = p.res ? dt<T>::ld((const T *)p.res + row * p.res_ld + e) : 0.f;
+                    return (x + res) * (double)g;
+                };
+                // the row's largest is among those within EDGE of fp32's
+                const float least = most < LEAST ? 0.f : most * (1.f - EDGE);
+                double exact = 0.;
+                if (live && own >= least) {
+                    unsigned long long near = 0;
+#pragma unroll
+                    for (int i = 0; i < VPT; i++) {
+                        const int v = tid + i * threads;
+                        float g[VN];
+                        if (v >= nv) continue;
+                        gain_of(i, v, g);
+#pragma unroll
+                        for (int j = 0; j < VN; j++)
+                            if (v * VN + j < p.C && fabsf(t[i][j] * g[j]) >= least) near |= 1ull << (i * VN + j);
+                    }
+                    each(near, [&](int, int e, float g) {
+                        exact = fmax(exact, fabs(exact_of(e, g)));
+                        return false;
+                    });
+                }
+                if (WARP) {
+                    for (int o = lanes / 2; o > 0; o >>= 1) exact = fmax(exact, __shfl_xor_sync(0xffffffffu, exact, o));
+                } else {
+                    if (exact > 0.) atomicMax(&largest, (unsigned long long)__double_as_longlong(exact));  // (doubles above zero are in the order of their bits)
+                    __syncthreads();
+                    exact = __longlong_as_double((long long)largest);
+                }
+                if (all && tid == 0 && live) p.q_scale[row] = (float)((double)r * (exact / 448.));
+                if (marks) {
+                    exact = 448. / exact;
+                    each(marks, [&](int, int e, float g) {
+                        p.q[row * p.q_ld + e] = (uint8_t)e4m3_of(exact_of(e, g) * exact);
+                        return true;
+                    });
+                }
+            }
         }
         if (!live) continue;
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
             const int v = tid + i * threads;
-            if (v >= (Q ? nvq : nv)) continue;
+            if (v >= nv) continue;
             float g[VN], w[VN];
             gain_of(i, v, g);
-            if (Q) {
-                uint32_t c[VN / 4];
-#pragma unroll
-                for (int j = 0; j < VN; j += 4) {
-#pragma unroll
-                    for (int k = 0; k < 4; k++) w[k] = t[i][j + k] * g[j + k] * code;
-                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(w[0], w[1]), __NV_SATFINITE, __NV_E4M3);
-                    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(w[2], w[3]), __NV_SATFINITE, __NV_E4M3);
-                    c[j / 4] = lo | hi << 16;
-                }
-                uint8_t *at = p.q + row * p.q_ld + v * VN;
-                if (VN == 4) *reinterpret_cast<uint32_t *>(at) = c[0];
-                else *reinterpret_cast<uint2 *>(at) = make_uint2(c[0], c[VN / 4 - 1]);
-            }
-            if (p.y && v < nv) {
+            if (Q && p.sum) *reinterpret_cast<uint4 *>((T *)p.sum + row * p.sum_ld + v * VN) = Vec16<T>::pack(t[i]);
+            if (p.y) {
 #pragma unroll
                 for (int j = 0; j < VN; j++) w[j] = t[i][j] * r * g[j];
                 if ((v + 1) * VN > p.C)  // (zeros behind the row, whatever r is)
