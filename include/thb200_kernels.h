@@ -17,7 +17,9 @@
  * Threading: the launch functions keep small host-side caches (TMA descriptors by buffer
  * and shape, per-device kernel attributes) without locks, as the reference's engines
  * keep their state: call them from one host thread at a time.  Everything they enqueue
- * goes to the stream they are given; nothing synchronises the device.
+ * goes to the stream they are given; nothing synchronises the device.  The weights of thb_conv_fwd and thb_gemv_fwd may be read while the
+ * launch before is still running: what lays them out has to be waited for (an event, a synchronisation) before the first call that uses
+ * them.  Everything else, the weights of thb_gemv_q4_fwd among it, may be what the launch before in the stream writes.
  */
 #ifndef THB200_KERNELS_H
 #define THB200_KERNELS_H
@@ -354,9 +356,7 @@ int thb_rmsnorm_fwd(const thb_rmsnorm_desc *d, const void *x, const void *res, v
  * code[m][k] is the low (k even) or high (k odd) nibble of byte k / 2 of row m of w.  x has the descriptor's dtype, or, where
  * x_scale is given, e4m3 codes with a scale a row, as thb_rmsnorm_fwd leaves them (and a dtype of y of any of the three).
  * Products are exact (fp32 x: in three parts), sums fp32.  What lies behind K in x and w is ignored; values of y behind M up
- * to the next multiple of the alignment are written as zeros.  w, wscale and wzero may be read as soon as the launch before this one in
- * the stream has ended or lets dependent launches start (programmatic dependent launch): a kernel of the caller's own that does
- * so early must have written them by then.  Kernels of this library do not write them. */
+ * to the next multiple of the alignment are written as zeros. */
 typedef struct thb_gemv_q4_desc {
     int dtype; /* F32 / F16 / BF16: of y, and of x without x_scale */
     int N, K, M;

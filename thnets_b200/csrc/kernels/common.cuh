@@ -12,6 +12,8 @@ extern "C" int thb_note_launch(cudaError_t e, const char *what);
 
 // Programmatic dependent launch.  A kernel launched by thb_launch may be set up while its predecessor in the stream still runs:
 // it calls pdl_enter() before its first access to global memory.  (THB200_PDL=0 launches plainly; pdl_enter is then free.)
+// Three kernels ask for weights ahead of that wait, which alone makes visible what the launch before has written: gemv.cu, conv_few_tc.cu
+// and conv_f32_tc.cu.  What lays such weights out has to be waited for before the first call (the engine's plans do).
 __device__ __forceinline__ void pdl_enter()
 {
     asm volatile("griddepcontrol.wait;" ::: "memory");

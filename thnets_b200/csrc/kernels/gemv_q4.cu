@@ -7,10 +7,14 @@
 // A code becomes q - z in 16 bits exactly (an integer of 5 bits): or'ed into the mantissa of 1024 (fp16; bf16: 128), then z + 1024 is
 // subtracted.  Products and their sums are exact or fp32, a group's sum takes its scale in fp32.  x in fp32 is three bf16 parts
 // (8 + 8 + 8 bits), each multiplied; e4m3 codes are fp16 numbers.
-// What bounds it: 9 (fp16) or 11 (bf16) instructions unpack 8 weights, as many again do everything else, and sixteen warps of 128 registers
-// issue in 40 to 55 % of the cycles only (waits for a stage, for shared memory, for warps with a tile more).  us a call in a chain (of the measured copy rate): 4096->128000, one row, bf16 groups of 128 53.9
-// (5.0 TB/s, 77 %); 4096->32003, four rows of e4m3, groups of 32 28.2 (43 %); 14336->4096, one row, fp16 11.4 (41 %); 9216->4096, eight rows,
-// bf16 groups of 64 with zero points 10.4 (31 %); 25088->4096, three rows, fp32 32.3 (25 %: most of its instructions take x apart).
+// What bounds it: waiting, with four warps to a scheduler (sixteen of 128 registers).  9 (fp16) or 11 (bf16) instructions unpack 8 weights and as
+// many again do everything else, 12 us of issue for the 4096->32003 below, but issue is busy in 32 to 53 % of the cycles only, the integer pipe in
+// 25 to 49 %.  Where rows are few a warp has 2 to 7 blocks in all: the latency of its first stage (the second is not asked for until x is staged),
+// of scales that are asked for two blocks ahead, and of the parts' exchange is most of the time; of the 4096->32003's 8.7 cycles an instruction 1.8 are
+// the exchange's barriers and 1.6 global loads.  us a call in a chain (of the measured copy rate): 4096->128000, one row, bf16 groups of 128 55.2
+// (4.9 TB/s, 75 %); 4096->32003, four rows of e4m3, groups of 32 25.6 (44 %); 14336->4096, one row, fp16 11.1 (42 %); 9216->4096, eight rows,
+// bf16 groups of 64 with zero points 10.8 (30 %); 25088->4096, three rows, fp32 33.6 (24 %: each row's values are three parts and three products,
+// on five empty columns of eight).  Variants for fp32 rows beyond the shared memory and zero points spill 200 to 376 bytes of registers.
 // Before: codes straight from global memory into registers 164 us for the 4096->32003, x in registers and tiles of 16 rows 31.  Tried and
 // slower: an equal share of a CTA's blocks for each warp, across tiles (a block or two less a warp, but 0.2 to 4 us more a call for where parts
 // begin and how they are joined); fp32 vectors taken apart by a warp's lanes together and handed on through shared memory (36 for 32).
@@ -282,10 +286,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
         const long at = row * p.s_ld + group;
         const uint8_t *z = ZEROS ? p.wzero + row * p.z_ld + group : nullptr;
         if (cut.wide == 2 && left >= SG) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)p.wscale + at));
+            const uint4 v = *reinterpret_cast<const uint4 *>((const uint16_t *)p.wscale + at);
             sn[0] = v.x; sn[1] = v.y; sn[2] = v.z; sn[3] = v.w;
             if (ZEROS) {
-                const uint2 u = __ldg(reinterpret_cast<const uint2 *>(z));
+                const uint2 u = *reinterpret_cast<const uint2 *>(z);
                 zn[0] = u.x; zn[1] = u.y;
             }
         } else if (cut.wide && NG > 1) {
@@ -294,20 +298,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
                 if (n * NG >= left) break;
                 const uint16_t *s = (const uint16_t *)p.wscale + at + n * NG;
                 if constexpr (NG == 4) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(s));
+                    const uint2 v = *reinterpret_cast<const uint2 *>(s);
                     sn[2 * n] = v.x; sn[2 * n + 1] = v.y;
-                    if (ZEROS) zn[n] = __ldg(reinterpret_cast<const uint32_t *>(z + n * NG));
+                    if (ZEROS) zn[n] = *reinterpret_cast<const uint32_t *>(z + n * NG);
                 } else {
-                    sn[n] = __ldg(reinterpret_cast<const uint32_t *>(s));
-                    if (ZEROS) zn[n] = __ldg(reinterpret_cast<const uint16_t *>(z + n * NG));
+                    sn[n] = *reinterpret_cast<const uint32_t *>(s);
+                    if (ZEROS) zn[n] = *reinterpret_cast<const uint16_t *>(z + n * NG);
                 }
             }
         } else {
 #pragma unroll
             for (int i = 0; i < SG; i++)
                 if (i < left) {
-                    sn[i] = p.s_dtype == THB_F32 ? __ldg((const uint32_t *)p.wscale + at + i) : __ldg((const uint16_t *)p.wscale + at + i);
-                    if (ZEROS) zn[i] = __ldg(z + i);
+                    sn[i] = p.s_dtype == THB_F32 ? ((const uint32_t *)p.wscale)[at + i] : ((const uint16_t *)p.wscale)[at + i];
+                    if (ZEROS) zn[i] = z[i];
                 }
         }
     };
@@ -355,11 +359,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gemv_q4_kernel(Q4Params p, Q4Cu
     const int xstep = g < p.N ? p.N * 4 : 0;
     const uint4 *const xmine = g < p.N ? xs + g * 4 + t : xs + blocks * 4 * X::PARTS * p.N * 4;
 
-    // The weights do not depend on the launch before this one: the first stage is under way while that one drains (a chain of 4096->4096 fp16 on one
-    // row from HBM 5.9 -> 5.3 us a call, 9216->4096 bf16 on eight 12.1 -> 11.0; brought as far as the L2 only: no gain).
+    // Codes, scales and zero points may be what the launch before has written, which only the wait in pdl_enter() makes visible: nothing of them
+    // is read ahead of it, and none through the non-coherent path, whose data has to stay as it is for as long as a kernel runs.
+    pdl_enter();
     fetch();
     fetch_scales(tile0 + mw, b0);
-    pdl_enter();
     if constexpr (XS) {
         for (int e = tid; e < blocks * 16 * p.N; e += WARPS * 32) {
             const int tt = e & 3, n = (e >> 2) % p.N, i = (e >> 2) / p.N & 3, b = (e >> 2) / p.N >> 2, k = x_at(b, i, tt);
