@@ -23,6 +23,6 @@ def test_nothing_is_read_ahead_of_the_wait(name, ahead):
             assert use not in body or body.index(use) > wait, (name, use)
 
 
-@pytest.mark.parametrize("name", ["gemv_q4.cu", "kv_append.cu"])
+@pytest.mark.parametrize("name", ["gemv_q4.cu", "rmsnorm.cu", "kv_append.cu", "paged_attn.cu"])
 def test_nothing_is_read_through_the_non_coherent_path(name):
     assert not re.search(r"__ldg|ld\.global\.nc|__restrict__", source(name))

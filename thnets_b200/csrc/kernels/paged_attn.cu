@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
     const int *table = p.c.table + (long)((unsigned)seq < (unsigned)p.c.sequences ? seq : 0) * p.c.table_ld;
     const bool whole = p.c.page_len % 16 == 0;
     const long start = (long)chunk * p.chunk + warp * 16 + (whole ? 0 : lane & 15);
-    int fpage = !p.window && start < (long)p.c.table_ld * p.c.page_len ? __ldg(table + (int)start / p.c.page_len) : 0;
+    int fpage = !p.window && start < (long)p.c.table_ld * p.c.page_len ? table[(int)start / p.c.page_len] : 0;
     int first, last;
     positions(p, row, first, last);
     if (last < first) return;
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(Shape<T, DP, HT>::WARPS * 32, Shape<T, DP, HT>
     // ---- a tile's loads.  Its page is looked up a tile earlier: one for all of it, or one a token (lane) where tiles cross pages
     auto page_of = [&](int tile) {
         const int token = whole ? tile : tile + (lane & 15);
-        return token < end ? __ldg(table + token / p.c.page_len) : 0;
+        return token < end ? table[token / p.c.page_len] : 0;
     };
     constexpr int COPIES = PIECES / 2;  // of 32 pieces
     auto row_of = [&](int i) { return (i * 32 + lane) / PIECES; };

@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, !Q ? 0 : WARP ? 4 : VPT <= 2
             for (int j = 0; j < VN; j++) g[j] = kept[KEEP ? i : 0][j];
         } else if constexpr (S::GLOBAL) {
 #pragma unroll
-            for (int j = 0; j < VN; j++) g[j] = p.gain && v * VN + j < p.C ? __ldg(p.gain + v * VN + j) : 1.f;
+            for (int j = 0; j < VN; j++) g[j] = p.gain && v * VN + j < p.C ? p.gain[v * VN + j] : 1.f;
         } else {
 #pragma unroll
             for (int j = 0; j < VN / 4; j++) {

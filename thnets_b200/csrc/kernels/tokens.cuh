@@ -1,4 +1,6 @@
 // What the operators of a decoder's step share: refusals, vectors of 16 bytes as floats, the device's SM count.
+// Whatever they are given (tables, scales, gains, weights) may be what the launch before writes: it is read behind pdl_enter(), by ordinary loads, since
+// the non-coherent ones (__ldg) are for what stays as it is from a kernel's start on, and a kernel may be started under the launch before.
 #pragma once
 #include "common.cuh"
 
