@@ -336,9 +336,9 @@ int thb_conv_u8_fwd_static(const thb_conv_desc *d, const void *x, void *y, thb_s
  *     t = x + res (res NULL: t = x);  sum = t;  v = t / sqrt(mean(t^2) + eps) * gain;  y = v;  q = e4m3(v / q_scale),
  *     q_scale = max|v| / 448 of the row.
  * sum, y and q (with q_scale) are optional, one of them at least is given; the norm is taken from t before it is rounded for
- * `sum`.  sum, y may be x or res themselves.  Values behind C up to the next multiple of the alignment are ignored in x and
- * res and written as zeros.  Codes are those of the quotient in exact arithmetic, rounded to fp32 and that to e4m3 (ties to even).  A
- * row whose v are all below 2^-100 has q_scale = 0 and zeros in q; one with an infinite or NaN t, or a norm beyond fp32's range (a sum
+ * `sum`.  sum, y may be x or res themselves, with the same ld; nothing else may overlap.  Values behind C up to the next multiple of the
+ * alignment are ignored in x and res and written as zeros.  Codes are those of the quotient in exact arithmetic, rounded to fp32 and that
+ * to e4m3 (ties to even).  A row whose v are all below 2^-100 has q_scale = 0 and zeros in q; one with an infinite or NaN t, or a norm beyond fp32's range (a sum
  * of t^2 above 2^128, whose y are then zero or NaN), has q_scale = NaN.  C <= 32768. */
 typedef struct thb_rmsnorm_desc {
     int dtype; /* F32 / F16 / BF16: of x, res, sum, y */
@@ -411,7 +411,7 @@ int thb_rope_freq_host(int dim, double base, int scaling, double factor, double 
                        double *freq_host, float *magnitude);
 
 /* New tokens into the cache: token t's keys, rotated by pos[t], and its values go to position pos[t] of sequence seq[t]; its queries,
- * rotated the same, to q_out (which may be q).  k, v, q: rows of heads * dim values (parts of one row of q, k and v side by
+ * rotated the same, to q_out (which may be q, with the same ld).  k, v, q: rows of heads * dim values (parts of one row of q, k and v side by
  * side, if the caller likes).  k = v = NULL: only the queries (the cache's dtype and dim are read, no more); q = q_out = NULL: only
  * the cache.  A token with pos < 0 is a place in a padded batch: nothing of it is written.  No two tokens of a call may have the
  * same position of the same sequence, nor two sequences of a call the same page where both write. */

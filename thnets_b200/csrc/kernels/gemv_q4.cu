@@ -603,6 +603,7 @@ extern "C" int thb_gemv_q4_fwd(const thb_gemv_q4_desc *d, const void *x, const f
     const int al = thb_channel_align(d->dtype), xal = x_scale ? 16 : al, groups = (d->K + d->group - 1) / d->group;
     if (thb_misaligned(x) || thb_misaligned(y) || thb_misaligned(d->w))
         return thb_refuse(THB_ERR_ARG, "thb_gemv_q4_fwd: x, y or w is not 16-byte aligned");
+    if (x == y) return thb_refuse(THB_ERR_ARG, "thb_gemv_q4_fwd: y in the place of x");
     if (d->x_ld % xal || d->x_ld < d->K || d->y_ld % al || d->y_ld < d->M)
         return thb_refuse(THB_ERR_ARG, "thb_gemv_q4_fwd: x_ld or y_ld is below the row or no multiple of the alignment");
     if (d->w_ld % 16 || d->w_ld < (d->K + 1) / 2 || d->s_ld < groups || (d->wzero && d->z_ld < groups))

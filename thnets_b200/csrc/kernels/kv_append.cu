@@ -224,6 +224,7 @@ extern "C" int thb_kv_append_fwd(const thb_kv_append_desc *d, const void *k, con
     const long kw = (long)d->cache.heads * dim, qw = (long)d->q_heads * dim;
     if (q && (d->q_heads < 1 || d->q_ld < qw || d->q_out_ld < qw || d->q_ld % al || d->q_out_ld % al || thb_misaligned(q) || thb_misaligned(q_out)))
         return thb_refuse(THB_ERR_ARG, "thb_kv_append_fwd: q_heads < 1, q or q_out not 16-byte aligned, or q_ld or q_out_ld below the row or no multiple of the alignment");
+    if (q && q == q_out && d->tokens > 1 && d->q_ld != d->q_out_ld) return thb_refuse(THB_ERR_ARG, "thb_kv_append_fwd: q_out in the place of q with another ld");
     if (k && (d->k_ld < kw || d->v_ld < kw || d->k_ld % al || d->v_ld % al || thb_misaligned(k) || thb_misaligned(v)))
         return thb_refuse(THB_ERR_ARG, "thb_kv_append_fwd: k or v not 16-byte aligned, or k_ld or v_ld below the row or no multiple of the alignment");
     // (a row's items are counted in 32 bits)

@@ -399,6 +399,10 @@ extern "C" int thb_rmsnorm_fwd(const thb_rmsnorm_desc *d, const void *x, const v
     for (const auto &e : t)
         if (e.p && (thb_misaligned(e.p) || e.ld % e.al || e.ld < d->C))
             return thb_refuse(THB_ERR_ARG, "thb_rmsnorm_fwd: a tensor is not 16-byte aligned, or its ld is below C or no multiple of the alignment");
+    // in place row by row only, and no two results in one place
+    auto moved = [&](const void *out, int ld) { return out && d->rows > 1 && ((out == x && ld != d->x_ld) || (out == res && ld != d->res_ld)); };
+    if (moved(sum, d->sum_ld) || moved(y, d->y_ld) || (sum && sum == y) || (q && (q == x || q == res || q == sum || q == y)))
+        return thb_refuse(THB_ERR_ARG, "thb_rmsnorm_fwd: a result in the place of an input with another ld, two results in one place, or q in the place of another tensor");
     const NormParams p = {x, res, sum, y, (uint8_t *)q, q_scale, d->gain, d->rows, d->C, d->x_ld, d->res_ld, d->sum_ld, d->y_ld, d->q_ld, d->eps};
     switch (d->dtype) {
     case THB_F32: return q ? launch_rmsnorm<float, true>(p, (cudaStream_t)s) : launch_rmsnorm<float, false>(p, (cudaStream_t)s);
