@@ -60,7 +60,7 @@ template <typename T, int U, bool INTER> struct AppendShape {
 template <typename T, int U, bool INTER>
 __global__ void __launch_bounds__(256, (AppendShape<T, U, INTER>::BLOCKS)) kv_append_kernel(AppendParams p, int items, int per, int slots, int parts)
 {
-    constexpr int HEADS = AppendShape<T, U, INTER>::HEADS, PAIRS = U == 1 ? 1 : INTER ? U / 2 : U;  // pairs an item
+    constexpr int HEADS = AppendShape<T, U, INTER>::HEADS, PAIRS = INTER ? U / 2 : U;  // pairs an item
     __shared__ float2 turns_of[8][128];
     pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(256, (AppendShape<T, U, INTER>::BLOCKS)) kv_ap
     const int token = (int)(mine / parts), part = (int)(mine % parts);
     if (token >= p.tokens) return;
     const int pos = p.pos[token], seq = p.k && p.seq ? p.seq[token] : token;
-    const int rot = p.rope.dim, half = rot / 2, dim = p.c.dim, turned = INTER ? (U == 1 ? half : rot / U) : half / U;
+    const int rot = p.rope.dim, half = rot / 2, dim = p.c.dim, turned = INTER ? rot / U : half / U;
     const int nq = p.q ? p.q_heads : 0, nk = p.k ? p.c.heads : 0, heads = nq + 2 * nk;
     const T *const q = (const T *)p.q + (long)token * p.q_ld, *const k = (const T *)p.k + (long)token * p.k_ld, *const v = (const T *)p.v + (long)token * p.v_ld;
     T *const q_out = (T *)p.q_out + (long)token * p.q_out_ld, *ck = nullptr, *cv = nullptr;
@@ -78,9 +78,9 @@ __global__ void __launch_bounds__(256, (AppendShape<T, U, INTER>::BLOCKS)) kv_ap
     for (int item0 = 0; item0 < items; item0 += per) {
         const int item = item0 + lane % per, sub = lane / per;
         const bool turns = item < turned, working = item < items && sub < slots;
-        // the item's first values, and those `apart` behind them where it has two units (interleaved single values: the pair's other one)
-        const int at = turns ? (INTER && U == 1 ? 2 * item : item * U) : rot + (item - turned) * U;
-        const int apart = !turns ? 0 : !INTER ? half : U == 1 ? 1 : 0;
+        // the item's first values, and those `apart` behind them where it has two units
+        const int at = turns ? item * U : rot + (item - turned) * U;
+        const int apart = turns && !INTER ? half : 0;
         float2 w[PAIRS];
         for (int h0 = part * slots + sub; h0 - sub < heads; h0 += HEADS * slots * parts) {
             Unit<T, U> a[HEADS], b[HEADS];
@@ -128,20 +128,20 @@ __global__ void __launch_bounds__(256, (AppendShape<T, U, INTER>::BLOCKS)) kv_ap
                 if (turns && h < nq + nk) {
                     float x[U], y[U];
                     a[i].unpack(x);
-                    if (!INTER || U == 1) {
+                    if constexpr (!INTER) {
                         b[i].unpack(y);
 #pragma unroll
                         for (int j = 0; j < U; j++) {
-                            const float r = x[j] * w[j % PAIRS].x - y[j] * w[j % PAIRS].y;
-                            y[j] = x[j] * w[j % PAIRS].y + y[j] * w[j % PAIRS].x;
+                            const float r = x[j] * w[j].x - y[j] * w[j].y;
+                            y[j] = x[j] * w[j].y + y[j] * w[j].x;
                             x[j] = r;
                         }
                         b[i].pack(y);
                     } else {
 #pragma unroll
-                        for (int j = 0; j + 1 < U; j += 2) {
-                            const float r = x[j] * w[j / 2 % PAIRS].x - x[j + 1] * w[j / 2 % PAIRS].y;
-                            x[j + 1] = x[j] * w[j / 2 % PAIRS].y + x[j + 1] * w[j / 2 % PAIRS].x;
+                        for (int j = 0; j < U; j += 2) {
+                            const float r = x[j] * w[j / 2].x - x[j + 1] * w[j / 2].y;
+                            x[j + 1] = x[j] * w[j / 2].y + x[j + 1] * w[j / 2].x;
                             x[j] = r;
                         }
                     }
@@ -159,14 +159,14 @@ template <typename T, int U> int launch_units(const AppendParams &p, cudaStream_
     const int rot = p.rope.dim, half = rot / 2, dim = p.c.dim, heads = (p.q ? p.q_heads : 0) + (p.k ? 2 * p.c.heads : 0);
     const bool inter = p.rope.interleaved;
     // a head's items, taken at most 32 at a time
-    const int items = (inter ? (U == 1 ? half : rot / U) : half / U) + (dim - rot) / U, turns = (items + 31) / 32, per = (items + turns - 1) / turns, slots = 32 / per;
+    const int items = (inter ? rot / U : half / U) + (dim - rot) / U, turns = (items + 31) / 32, per = (items + turns - 1) / turns, slots = 32 / per;
     // a warp a token where there are enough of them for 16 warps an SM; else as many as that takes, with a few heads each
     long parts = 1;
     const int most = (heads + slots - 1) / slots;
     while (parts * 2 <= most && p.tokens * parts < 16 * 148L) parts *= 2;
     const unsigned grid = (unsigned)((p.tokens * parts + 7) / 8);
-    if (inter) thb_launch(kv_append_kernel<T, U, true>, grid, 256, st, p, items, per, slots, (int)parts);
-    else thb_launch(kv_append_kernel<T, U, false>, grid, 256, st, p, items, per, slots, (int)parts);
+    if (!inter) thb_launch(kv_append_kernel<T, U, false>, grid, 256, st, p, items, per, slots, (int)parts);
+    else if constexpr (U > 1) thb_launch(kv_append_kernel<T, U, true>, grid, 256, st, p, items, per, slots, (int)parts);  // (pairs are whole in units of two)
     return THB_LAUNCH_CHECK("kv_append_kernel");
 }
 
