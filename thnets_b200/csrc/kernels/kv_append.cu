@@ -6,7 +6,9 @@
 // latency-bound on a decoder's single tokens.
 // us a launch in a chain (share of the measured copy rate), 8192 tokens of 32 + 8 + 8 heads: of 128 in bf16, halves 36.6 (84 %); half of each
 // turned in neighbouring pairs, fp16 37.5 (82 %); of 64 23.3 (66 %); 4096 tokens in fp32 34.7 (89 %).  With a block to a token, which
-// waits for the angles together: 56 / 47 / 34 / 36.
+// waits for the angles together: 56 / 47 / 34 / 36.  One unit serves all of a token's values, the unturned ones and v too: with halves that are
+// no whole vectors, all travel in 8, 4 or 2 bytes (4096 tokens of 36 heads of 80 in bf16, 40 / 20 / 10 values turned: 22.5 / 41.8 / 57.6, bytes
+// alone 7.2).
 #include "tokens.cuh"
 #include <math.h>
 
@@ -52,7 +54,8 @@ template <typename T, int U> struct Unit {
 // How many heads, and blocks an SM.  Halves in whole units: few warps with many loads each (8192 tokens of 32 + 8 + 8 heads of 128 in bf16, 6 and
 // two blocks against 4 and two: 36.6 us for 39.8).  Pairs, or smaller units, take more instructions a byte: fewer loads, more warps (half of each
 // head in pairs, fp16, 3 and four against 4 and three: 37.5 for 40.3; 4096 tokens of 36 heads of 80 in units of 8 bytes, 2 and four against 4 and
-// three: 22.0 for 35.7; of single values it loses, 56.6 for 51).
+// three: 22.0 for 35.7).  Halves of an odd number of values, taken one by one, 2 and four against 4 and three: 4096 tokens of 36 heads of 80 with 10 values
+// turned 57.6 for 62.6 in bf16, 57.7 for 67.3 in fp32, 512 of them 10.6 for 12.2; 8192 of 48 heads of 128 with 18 turned 170 for 163.
 template <typename T, int U, bool INTER> struct AppendShape {
     static constexpr bool MANY = !INTER && sizeof(T) * U == 16;
     static constexpr int HEADS = INTER ? 3 : MANY ? 6 : 2, BLOCKS = MANY ? 2 : 4;
