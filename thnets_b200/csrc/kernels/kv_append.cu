@@ -166,7 +166,7 @@ template <typename T, int U> int launch_units(const AppendParams &p, cudaStream_
     // a warp a token where there are enough of them for 16 warps an SM; else as many as that takes, with a few heads each
     long parts = 1;
     const int most = (heads + slots - 1) / slots;
-    while (parts * 2 <= most && p.tokens * parts < 16 * 148L) parts *= 2;
+    while (parts * 2 <= most && p.tokens * parts < 16L * thb_sm_count()) parts *= 2;
     const unsigned grid = (unsigned)((p.tokens * parts + 7) / 8);
     if (!inter) thb_launch(kv_append_kernel<T, U, false>, grid, 256, st, p, items, per, slots, (int)parts);
     else if constexpr (U > 1) thb_launch(kv_append_kernel<T, U, true>, grid, 256, st, p, items, per, slots, (int)parts);  // (pairs are whole in units of two)

@@ -595,7 +595,8 @@ Cut cut_of(const thb_paged_attn_desc *d)
     const int share = d->q_heads / d->cache.heads;
     c.ht = d->cache.dtype == THB_F32 ? (share > 4 ? 8 : share > 2 ? 4 : share) : share > 8 && d->cache.dim <= 128 ? 16 : 8;
     c.head_tiles = (share + c.ht - 1) / c.ht;
-    // One wave of CTAs on a B200's 148 SMs (as many to each as Shape says) where the rows are max_len long; a tile for each of four warps at
+    // One wave of CTAs on a B200's 148 SMs (a constant: the size of scratch and the bits of the results do not depend on the device that is current;
+    // as many CTAs to each SM as Shape says) where the rows are max_len long; a tile for each of four warps at
     // least.  Of several rows a CTA takes 2048 tokens at most, so that a few long ones among short ones are still many CTAs.
     const int row_bytes = d->cache.dim * (d->cache.dtype == THB_F32 ? 4 : 2), slots = 148 * (row_bytes <= 128 ? 4 : row_bytes <= 512 ? 2 : 1);
     const double base = (double)d->rows * d->cache.heads * c.head_tiles;
