@@ -405,7 +405,9 @@ typedef struct thb_rope {
 /* freq and magnitude of the usual scalings: freq[i] = base^(-2i/dim), and for contexts `factor` times longer than a model was trained for
  * LINEAR: divided by factor (positions interpolated); BASE: base multiplied by factor^(dim/(dim-2)) (the "NTK-aware" base);
  * BY_PARTS: divided by factor where a pair makes at most slow_turns turns in trained_len positions, kept where it makes
- * fast_turns or more, in proportion between, and magnitude 0.1 ln(factor) + 1 (YaRN).  The other scalings' magnitude is 1. */
+ * fast_turns or more, between in proportion to the turns, and magnitude 0.1 ln(factor) + 1 (YaRN as published; programs that go by the
+ * pair's number between two rounded bounds instead have other frequencies there, which a caller fills in itself).  The other scalings'
+ * magnitude is 1. */
 enum { THB_ROPE_PLAIN = 0, THB_ROPE_LINEAR = 1, THB_ROPE_BASE = 2, THB_ROPE_BY_PARTS = 3 };
 int thb_rope_freq_host(int dim, double base, int scaling, double factor, double trained_len, double slow_turns, double fast_turns,
                        double *freq_host, float *magnitude);
