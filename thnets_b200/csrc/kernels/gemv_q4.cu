@@ -12,7 +12,7 @@
 // 25 to 49 %.  Where rows are few a warp has 2 to 7 blocks in all: the latency of its first stage (the second is not asked for until x is staged),
 // of scales that are asked for two blocks ahead, and of the parts' exchange is most of the time; of the 4096->32003's 8.7 cycles an instruction 1.8 are
 // the exchange's barriers and 1.6 global loads.  us a call in a chain (of the measured copy rate): 4096->128000, one row, bf16 groups of 128 55.2
-// (4.9 TB/s, 75 %); 4096->32003, four rows of e4m3, groups of 32 25.6 (44 %); 14336->4096, one row, fp16 11.1 (42 %); 9216->4096, eight rows,
+// (4.9 TB/s, 75 %); 4096->32003, four rows of e4m3, groups of 32 with zero points 29.8 (40 %); 14336->4096, one row, fp16 11.1 (42 %); 9216->4096, eight rows,
 // bf16 groups of 64 with zero points 10.8 (30 %); 25088->4096, three rows, fp32 33.6 (24 %: each row's values are three parts and three products,
 // on five empty columns of eight).  Variants for fp32 rows beyond the shared memory and zero points spill 200 to 376 bytes of registers.
 // Before: codes straight from global memory into registers 164 us for the 4096->32003, x in registers and tiles of 16 rows 31.  Tried and

@@ -5,8 +5,9 @@
 // rounding does not reach the codes.  HBM-bound on many rows, and near it by the instructions a value takes; latency-bound on few.
 // us a launch in a chain (share of the measured copy rate): 8192 rows of 4096 in fp16 with residual 43.3 (95 %), without residual 26.9 (76 %);
 // 4096 of 8192 42.8 (96 %); 2048 of 16384 60 (68 %); 262144 of 128 30.6 (67 %); 8192 of 4096 in fp32 90 (91 %).  To e4m3, whose codes are
-// settled as below: 8192 of 4096 in bf16 with residual 58.6 (61 %; 41.0 with codes that the roundings of fp32 decide), fp32 81.0 (82 %, 76.9),
-// without residual 44.7 (34 %, 33.1), 262144 of 128 without 41.2 (38 %, 32.1), 2048 of 16384 79 (45 %, 55.2), 1024 of 32768 in fp32 160 (42 %, 138).
+// settled as below: 8192 of 4096 in bf16 with residual 49.8 (72 %; 41.1 with codes that the roundings of fp32 decide), y besides 56.2 (82 %, 57.5),
+// fp32 81.5 (82 %, 76.9), bf16 without residual 41.3 (37 %, 33.2), 262144 of 128 without 41.3 (38 %, 32.0), 30000 of 1000 in fp16 53 (61 %, 42),
+// 4096 of 8192 61 (58 %, 41), 2048 of 16384 79 (45 %, 55), 1024 of 32768 in fp32 162 (42 %, 138).
 #include "tokens.cuh"
 #include <cuda_fp8.h>
 
@@ -36,8 +37,9 @@ __device__ __forceinline__ float max_nan(float a, float b)
 // maximum's roundings (three units; without a residual one, the maximum's); what that does not settle takes the row's maximum in exact
 // arithmetic, for which its threads come together once more.  Half of what it costs is the instructions of every row and the barrier that asks
 // whether any code is open, half the rows with such a value, 1 to 3 us each, of which one CTA has more than the others.  Tried and slower
-// (8192 of 4096 in bf16): the exact maximum of every row ahead of its first barrier 66 us; all that is rare out of line 124 (its calls spill the
-// row's registers); x and res kept in the ring until the row is done 68; rows with such values left for the end of the launch 61 (16384: 125).
+// (8192 of 4096 in bf16, four blocks an SM, 58.6 us): the exact maximum of every row ahead of its first barrier 66 us; all that is rare out of line
+// 124 (its calls spill the row's registers); x and res kept in the ring until the row is done 68; rows with such values left for the end of the launch
+// 61 (16384: 125).
 constexpr float EDGE = 8 * 0x1p-24f;
 // below this maximum 448 / max or the products leave fp32's range: all of the row's codes are settled in fp64
 constexpr float LEAST = 0x1p-100f;
@@ -59,8 +61,11 @@ template <typename T, int VPT, bool WARP> struct NormShape {
         return STAGES * VPT * threads * 16 * (res ? 2 : 1) + (KEEP || GLOBAL ? 0 : nvq * VN * 4);
     }
 };
-template <typename T, int VPT, bool WARP, bool Q>
-__global__ void __launch_bounds__(WARP ? 256 : 512, !Q ? 0 : WARP ? 4 : VPT <= 2 ? 2 : 1) rmsnorm_kernel(NormParams p, int lanes)
+// MOST: threads a block at most.  With codes the registers decide how many blocks stay on an SM: rows of two vectors for each of 256 threads take 80
+// and three blocks (8192 rows of 4096 in bf16 with residual: 49.7 us; in 64, which spill, and four 58.6), of up to 512 threads 64 and two (4096
+// rows of 8192: 61.2; four vectors for each of 256 threads 71.1), one vector a thread 64.
+template <typename T, int VPT, bool WARP, bool Q, int MOST>
+__global__ void __launch_bounds__(MOST, !Q ? 0 : WARP || VPT == 1 ? 1024 / MOST : VPT == 2 ? (MOST == 256 ? 3 : 2) : 1) rmsnorm_kernel(NormParams p, int lanes)
 {
     using S = NormShape<T, VPT, WARP>;
     constexpr int VN = S::VN, STAGES = S::STAGES;
@@ -329,10 +334,10 @@ __global__ void __launch_bounds__(WARP ? 256 : 512, !Q ? 0 : WARP ? 4 : VPT <= 2
     }
 }
 
-template <typename T, int VPT, bool Q> int launch_block(const NormParams &p, cudaStream_t st)
+template <typename T, int VPT, bool Q, int MOST = 512> int launch_block(const NormParams &p, cudaStream_t st)
 {
     using S = NormShape<T, VPT, false>;
-    const auto kern = rmsnorm_kernel<T, VPT, false, Q>;
+    const auto kern = rmsnorm_kernel<T, VPT, false, Q, MOST>;
     const int nvq = (p.C + 15) / 16 * (16 / S::VN), threads = ((nvq + VPT - 1) / VPT + 31) / 32 * 32, smem = S::smem(threads, nvq, p.res != nullptr);
     static int sms[64];
     int dev = 0;
@@ -344,9 +349,9 @@ template <typename T, int VPT, bool Q> int launch_block(const NormParams &p, cud
         sms[dev] = thb_sm_count();
     }
     // As many blocks as stay on the device at once, each with many rows: with two vectors a thread so many that 64 KB are under way an SM
-    // (8192 rows of 4096 in 16 bits with a residual: 43.6 us with two blocks of 256 threads, 52.8 with four; without one 30.5 and 26.9; to codes 46.4 and 41.1), with one
+    // (8192 rows of 4096 in 16 bits with a residual: 43.6 us with two blocks of 256 threads, 52.8 with four; without one 30.5 and 26.9), with one
     // as many as there is room for (30000 rows of 1000: 48.7 us with 1024 threads an SM, 40.8 with 2048).
-    const int by_smem = 220 * 1024 / (smem + 2048), by_threads = (VPT == 1 ? 2048 : VPT == 2 && (Q || !p.res) ? 1024 : 512) / threads, resident = by_smem < by_threads ? by_smem : by_threads;
+    const int by_smem = 220 * 1024 / (smem + 2048), by_threads = (VPT == 1 ? 2048 : VPT == 2 && Q ? (MOST == 256 ? 768 : 1024) : VPT == 2 && !p.res ? 1024 : 512) / threads, resident = by_smem < by_threads ? by_smem : by_threads;
     const long most = (long)(resident < 1 ? 1 : resident) * sms[dev];
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.rows < most ? p.rows : most));
@@ -370,10 +375,12 @@ template <typename T, bool Q> int launch_rmsnorm(const NormParams &p, cudaStream
         int lanes = 1;
         while (lanes < nv) lanes *= 2;
         const long blocks = (p.rows + 256 / lanes - 1) / (256 / lanes), most = 8L * thb_sm_count();
-        thb_launch(rmsnorm_kernel<T, 1, true, Q>, (unsigned)(blocks < most ? blocks : most), 256, st, p, lanes);
+        thb_launch(rmsnorm_kernel<T, 1, true, Q, 256>, (unsigned)(blocks < most ? blocks : most), 256, st, p, lanes);
         return THB_LAUNCH_CHECK("rmsnorm_kernel");
     }
-    if (nv <= 256) return launch_block<T, 1, Q>(p, st);
+    if (nv <= 256) return launch_block<T, 1, Q, 256>(p, st);
+    if constexpr (Q)
+        if (nv <= 512) return launch_block<T, 2, Q, 256>(p, st);
     if (nv <= 1024) return launch_block<T, 2, Q>(p, st);
     if (nv <= 2048) return launch_block<T, 4, Q>(p, st);
     if (nv <= 4096) return launch_block<T, 8, Q>(p, st);
