@@ -338,8 +338,9 @@ int thb_conv_u8_fwd_static(const thb_conv_desc *d, const void *x, void *y, thb_s
  * sum, y and q (with q_scale) are optional, one of them at least is given; the norm is taken from t before it is rounded for
  * `sum`.  sum, y may be x or res themselves, with the same ld; nothing else may overlap.  Values behind C up to the next multiple of the
  * alignment are ignored in x and res and written as zeros.  Codes are those of the quotient in exact arithmetic, rounded to fp32 and that
- * to e4m3 (ties to even).  A row whose v are all below 2^-100 has q_scale = 0 and zeros in q; one with an infinite or NaN t, or a norm beyond fp32's range (a sum
- * of t^2 above 2^128, whose y are then zero or NaN), has q_scale = NaN.  C <= 32768. */
+ * to e4m3 (ties to even).  A row whose v are all below 2^-100, or whose t * gain are all zero in fp32, has q_scale = 0 and zeros in q; one with
+ * an infinite or NaN t, or a norm beyond fp32's range (a sum of t^2 above 2^128, whose y are then zero or NaN), has q_scale = NaN.
+ * C <= 32768. */
 typedef struct thb_rmsnorm_desc {
     int dtype; /* F32 / F16 / BF16: of x, res, sum, y */
     int C;

@@ -47,7 +47,7 @@ def test_gemv_q4_of_what_the_launch_before_writes(lib, last, group, pad, dtype, 
         assert layer.call(lib, stream) == 0
         got.append(layer.y.clone())
     torch.cuda.synchronize()
-    for i in range(2):  # (the states of rounds 39 and 40 are those of every second round)
+    for i in range(2):  # (the states of the last two calls are those of every second one)
         layer.y.copy_(got[39 - i])
         z = layer.z
         layer.z = z & 15  # (the low four bits count)

@@ -1,5 +1,6 @@
 """The norm's e4m3 codes against the formula in 64 bits, code by code: v / q_scale rounded to fp32 and that to e4m3, however near it is to
-the border of two codes.  Rows made of borders, rows of ordinary values, rows too small for 448 / max|t * gain| in fp32."""
+the border of two codes.  Rows made of borders, few and so many that a block has several, rows of ordinary values, rows too small for
+448 / max|t * gain| in fp32."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -44,7 +45,8 @@ def outputs(rows, c, dtype):
 @pytest.mark.parametrize("dtype", EVERY)
 @pytest.mark.parametrize("with_res", [False, True])
 @pytest.mark.parametrize("with_gain", [False, True])
-@pytest.mark.parametrize("rows,c", [(513, 16), (300, 63), (129, 255), (300, 1004), (200, 4096), (40, 9000), (5, 20001), (3, 32768)])
+@pytest.mark.parametrize("rows,c", [(513, 16), (300, 63), (129, 255), (300, 1004), (200, 4096), (40, 9000), (5, 20001), (3, 32768),
+                                    (40001, 16), (20003, 255), (7001, 1004), (2501, 2500), (2003, 4096), (1001, 9000), (603, 20001), (401, 32768)])
 def test_codes_at_borders(lib, dtype, with_res, with_gain, rows, c):
     """Every value is a border of two codes, or beside one by a unit of fp32, by the gain or by what the residual adds."""
     td, al = TORCH[dtype], K.ALIGN[dtype]
